@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import contextlib
 import threading
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -564,6 +565,284 @@ def batchnorm2d_act(x, gamma, beta, run_mean, run_var, momentum=0.1,
     y = torch.nn.functional.batch_norm(x, run_mean, run_var, gamma, beta,
                                        training, momentum, eps)
     return torch.relu(y) if relu else y
+
+
+# -- dropout from a counter ---------------------------------------------------
+
+_FLOAT_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _check_float(name: str, t: torch.Tensor) -> None:
+    if t.dtype not in _FLOAT_TYPES:
+        raise ValueError("%s must be fp32, bf16 or fp16, got %s"
+                         % (name, t.dtype))
+
+
+def dropout_state(seed: int, offset: int = 0, device=None) -> torch.Tensor:
+    """The two 64-bit numbers that a dropout mask is drawn from: the
+    generator's key and the number of the draw."""
+    def signed(v):
+        return (int(v) + 2 ** 63) % 2 ** 64 - 2 ** 63
+
+    return torch.tensor([signed(seed), signed(offset)], dtype=torch.int64,
+                        device=device)
+
+
+def _check_state(state: torch.Tensor) -> None:
+    if state.dtype != torch.int64 or state.numel() != 2 \
+            or not state.is_contiguous():
+        raise ValueError("state must be two contiguous int64 (see "
+                         "dropout_state)")
+
+
+def dropout_next(state: torch.Tensor) -> torch.Tensor:
+    """The state for one draw; steps ``state`` on to the next draw in
+    place.  On a GPU both happen on the device in one launch, so a
+    captured step draws a new mask at each replay."""
+    _check_state(state)
+    if ops.use_hip(state):
+        return ops.hip.dropout_next(state)
+    out = state.clone()
+    state[1] += 1
+    return out
+
+
+def _mul32(a: int, c: torch.Tensor):
+    """(high, low) 32 bits of a * c for 32-bit values held in int64: the
+    product is taken in two halves of 48 bits, its low part modulo 2^64."""
+    high = (a * (c >> 16) + ((a * (c & 0xFFFF)) >> 16)) >> 16
+    return high, (a * c) & 0xFFFFFFFF
+
+
+def _philox_words(state: torch.Tensor, n: int) -> torch.Tensor:
+    """The first n words of the CPU path, in int64 (the GPU kernel's words;
+    see ops/hip/dropout.hip)."""
+    mask = 0xFFFFFFFF
+    seed, offset = (int(v) for v in state)
+    at = torch.arange((n + 3) // 4, dtype=torch.int64)
+    c0, c1 = at & mask, at >> 32
+    c2 = torch.full_like(at, offset & mask)
+    c3 = torch.full_like(at, (offset >> 32) & mask)
+    k0, k1 = seed & mask, (seed >> 32) & mask
+    for _ in range(10):
+        h0, l0 = _mul32(0xD2511F53, c0)
+        h1, l1 = _mul32(0xCD9E8D57, c2)
+        c0, c1, c2, c3 = h1 ^ c1 ^ k0, l1, h0 ^ c3 ^ k1, l0
+        k0, k1 = (k0 + 0x9E3779B9) & mask, (k1 + 0xBB67AE85) & mask
+    return torch.stack((c0, c1, c2, c3), 1).reshape(-1)[:n]
+
+
+class Dropout(torch.autograd.Function):
+    """The mask is a function of the state and the element's index; only
+    the state is kept, and backward draws the same mask again."""
+
+    @staticmethod
+    def forward(ctx, x, state, p: float):
+        ctx.save_for_backward(state)
+        ctx.p = p
+        keep = round((1.0 - p) * 2 ** 32)  # of 2^32 words
+        if keep == 0:
+            return torch.zeros_like(x, memory_format=torch.contiguous_format)
+        scale = 1.0 / (1.0 - p)
+        if ops.use_hip(x):
+            return ops.hip.dropout(x.contiguous(), state, keep, scale)
+        kept = (_philox_words(state, x.numel()) < keep).reshape(x.shape)
+        y = (x.to(torch.float32) * scale).to(x.dtype)
+        return torch.where(kept, y, torch.zeros_like(y))
+
+    @staticmethod
+    def backward(ctx, dy):
+        (state,) = ctx.saved_tensors
+        return Dropout.apply(dy, state, ctx.p), None, None
+
+
+def dropout(x, p: float, state, training: bool = True):
+    """Inverted dropout with a mask that is drawn from ``state`` (see
+    ``dropout_state`` and ``dropout_next``) and never stored.
+
+    An element is kept with probability 1 - p and scaled by 1 / (1 - p); a
+    dropped one is 0 whatever it held.  The same state gives the same mask
+    for the same number of elements, on any device, in any type.  x: fp32,
+    bf16 or fp16, any shape; other layouts than contiguous are copied.
+    Without ``training``, or with p = 0, x comes back as it is.
+    """
+    _check_float("x", x)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError("p must be within 0 and 1, got %r" % (p,))
+    _check_state(state)
+    if state.device != x.device:
+        raise ValueError("x is on %s and state on %s"
+                         % (x.device, state.device))
+    if not training or p == 0.0:
+        return x
+    return Dropout.apply(x, state, float(p))
+
+
+# -- log-probabilities of given tokens ----------------------------------------
+
+_TOP_MAX = 32
+
+
+class TokenLogProbs(NamedTuple):
+    """``logp`` and ``entropy``: one fp32 a row; ``top_logp`` (fp32) and
+    ``top_ids`` (int64): the ``top_k`` best classes, best first."""
+    logp: torch.Tensor
+    entropy: torch.Tensor
+    top_logp: torch.Tensor
+    top_ids: torch.Tensor
+
+
+class _TokenLogProbs(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, logits, tokens, k: int, ignore: int):
+        ctx.set_materialize_grads(False)
+        if ops.use_hip(logits):
+            logp, entropy, stat, top, ids = ops.hip.logprobs_fwd(
+                logits, tokens, k, ignore)
+        else:
+            logp, entropy, stat, top, ids = _logprobs_cpu(
+                logits, tokens.long(), k, ignore)
+        ctx.save_for_backward(logits, tokens, stat, entropy, ids)
+        ctx.ignore = ignore
+        ctx.mark_non_differentiable(ids)
+        return logp, entropy, top, ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logp, g_entropy, g_top, _):
+        logits, tokens, stat, entropy, ids = ctx.saved_tensors
+        gs = [None if g is None else g.contiguous()
+              for g in (g_logp, g_entropy, g_top)]
+        if ops.use_hip(logits):
+            dx = ops.hip.logprobs_bwd(logits, tokens, stat, entropy, ids,
+                                      *gs, ctx.ignore)
+        else:
+            dx = _logprobs_grad_cpu(logits, tokens.long(), stat, entropy,
+                                    ids, *gs, ctx.ignore)
+        return dx, None, None, None
+
+
+def _logprobs_cpu(logits, tokens, k, ignore):
+    x = logits.to(torch.float32)
+    m, c = x.shape
+    live = tokens != ignore
+    known = (tokens >= 0) & (tokens < c)
+    best = x.amax(1, keepdim=True)
+    # a row of -inf alone: no class is possible
+    empty = (best == -float("inf")).squeeze(1)
+    shift = torch.where(best == -float("inf"), torch.zeros_like(best), best)
+    log_sum = torch.exp(x - shift).sum(1, keepdim=True).log()
+    log_sum = torch.where(empty.unsqueeze(1), torch.zeros_like(log_sum),
+                          log_sum)
+    all_logp = torch.where(x == -float("inf"), x, (x - shift) - log_sum)
+    p = torch.where(empty.unsqueeze(1), torch.zeros_like(x),
+                    torch.exp(all_logp))
+    entropy = -torch.where(p == 0, torch.zeros_like(p), p * all_logp).sum(1)
+    logp = all_logp.gather(
+        1, torch.where(known, tokens, 0).unsqueeze(1)).squeeze(1)
+    logp = torch.where(known, logp, torch.full_like(logp, float("nan")))
+    ids = torch.sort(x, dim=1, descending=True, stable=True)[1][:, :k]
+    top = all_logp.gather(1, ids)
+    broken = torch.isnan(log_sum)  # a NaN or +inf: no distribution
+    logp = torch.where(broken.squeeze(1), log_sum.squeeze(1), logp)
+    top = torch.where(broken, log_sum, top)
+    ids = torch.where(broken, torch.full_like(ids, -1), ids)
+    # rows that are not read
+    logp, entropy = (torch.where(live, t, torch.zeros_like(t))
+                     for t in (logp, entropy))
+    top = torch.where(live.unsqueeze(1), top, torch.zeros_like(top))
+    ids = torch.where(live.unsqueeze(1), ids, torch.full_like(ids, -1))
+    return logp, entropy, torch.cat((best, log_sum), 1), top, ids
+
+
+def _logprobs_grad_cpu(logits, tokens, stat, entropy, ids, g_logp, g_entropy,
+                       g_top, ignore):
+    x = logits.to(torch.float32)
+    m, c = x.shape
+    live = (tokens != ignore).unsqueeze(1)
+    known = ((tokens >= 0) & (tokens < c)).unsqueeze(1)
+    one_hot = torch.zeros_like(x)
+    if g_logp is not None:
+        g = g_logp.unsqueeze(1)
+        g = torch.where(known, g, torch.full_like(g, float("nan")))
+        one_hot.scatter_add_(
+            1, torch.where(known.squeeze(1), tokens, 0).unsqueeze(1), g)
+    if g_top is not None:
+        one_hot.scatter_add_(1, ids.clamp(min=0), g_top)
+    share = one_hot.sum(1, keepdim=True)
+    best, log_sum = stat[:, :1], stat[:, 1:]
+    h = entropy.unsqueeze(1)
+    logp = (x - best) - log_sum
+    p = torch.exp(logp)
+    d = one_hot - p * share
+    if g_entropy is not None:
+        d = d - g_entropy.unsqueeze(1) * torch.where(
+            p == 0, torch.zeros_like(p), p * (logp + h))
+    if g_logp is not None:
+        d = torch.where(known, d, torch.full_like(d, float("nan")))
+    constant = (best == -float("inf")) & (log_sum == 0) & (
+        known if g_logp is not None else torch.ones_like(known))
+    d = torch.where(live & ~constant, d, torch.zeros_like(d))
+    return d.to(logits.dtype)
+
+
+def token_logprobs(logits, tokens, top_k: int = 0,
+                   ignore_index: int = -100) -> TokenLogProbs:
+    """Log-probability of one given class a row, with the entropy of the
+    row's distribution and its ``top_k`` best classes; gradients flow from
+    all three.
+
+    logits: [..., classes] in fp32, bf16 or fp16, read in place where the
+    classes lie side by side (rows may be strided, as in a slice of a
+    padded vocabulary).  tokens: the leading shape of logits, or that with
+    a last extent of 1 (the engine's labels); whole numbers in an integer
+    type or fp32.  ``top_k`` is at most 32 and the number of classes; of
+    equal logits the lower class is the better one.
+
+    * A row whose token is ``ignore_index`` is not read: zeros, top ids
+      of -1, and a gradient of zero.
+    * A token outside 0 .. classes - 1 cannot be refused without waiting
+      for the device: its log-probability is NaN, and so is its row of the
+      gradient if one flows from there.
+    * A logit of -inf has probability 0, adds nothing to the entropy and
+      takes no gradient through it.  A row of nothing else has -inf for
+      every class, an entropy of 0 and a gradient of zero.
+    * A row that holds NaN or +inf has no distribution: NaN everywhere and
+      top ids of -1.
+    """
+    _check_float("logits", logits)
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError("logits must be [..., classes], got %s"
+                         % (tuple(logits.shape),))
+    classes = logits.shape[-1]
+    if tokens.dim() == logits.dim() and tokens.shape[-1] == 1:
+        tokens = tokens.squeeze(-1)
+    if tokens.shape != logits.shape[:-1]:
+        raise ValueError("tokens of shape %s do not fit logits of shape %s"
+                         % (tuple(tokens.shape), tuple(logits.shape)))
+    if tokens.device != logits.device:
+        raise ValueError("logits are on %s and tokens on %s"
+                         % (logits.device, tokens.device))
+    if tokens.dtype == torch.bool or tokens.is_complex() or (
+            tokens.is_floating_point() and tokens.dtype != torch.float32):
+        raise ValueError("tokens must be whole numbers in an integer type "
+                         "or fp32, got %s" % (tokens.dtype,))
+    if not 0 <= top_k <= min(_TOP_MAX, classes):
+        raise ValueError("top_k must be within 0 and min(%d, %d classes), "
+                         "got %r" % (_TOP_MAX, classes, top_k))
+    shape = tokens.shape
+    rows = logits.reshape(-1, classes)
+    if rows.stride(1) != 1 and classes > 1:
+        rows = rows.contiguous()
+    tokens = tokens.detach().reshape(-1)
+    if tokens.dtype != torch.float32:
+        tokens = tokens.long()
+    logp, entropy, top, ids = _TokenLogProbs.apply(
+        rows, tokens.contiguous(), int(top_k), int(ignore_index))
+    return TokenLogProbs(logp.reshape(shape), entropy.reshape(shape),
+                         top.reshape(shape + (top_k,)),
+                         ids.reshape(shape + (top_k,)))
 
 
 def argmax_rows(y: torch.Tensor) -> torch.Tensor:

@@ -46,6 +46,23 @@ torch::Tensor mse_fwd(torch::Tensor pred, torch::Tensor target,
 torch::Tensor mse_bwd(torch::Tensor pred, torch::Tensor target,
                       torch::Tensor gscale, double mult);
 
+// dropout.hip — mask drawn from a counter, never stored
+torch::Tensor dropout(torch::Tensor x, torch::Tensor state, int64_t keep,
+                      double scale);
+torch::Tensor dropout_next(torch::Tensor state);
+
+// logprobs.hip — scores of given tokens, entropy, best alternatives
+std::vector<torch::Tensor> logprobs_fwd(torch::Tensor logits,
+                                        torch::Tensor tokens, int64_t k,
+                                        int64_t ignore);
+torch::Tensor logprobs_bwd(torch::Tensor logits, torch::Tensor tokens,
+                           torch::Tensor stat, torch::Tensor entropy,
+                           torch::Tensor ids,
+                           c10::optional<torch::Tensor> g_logp,
+                           c10::optional<torch::Tensor> g_entropy,
+                           c10::optional<torch::Tensor> g_top,
+                           int64_t ignore);
+
 // optim.hip
 void fused_sgd(torch::Tensor p, torch::Tensor g, double lr);
 void fused_momentum(torch::Tensor p, torch::Tensor g, torch::Tensor acc,
@@ -183,6 +200,19 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mse_fwd", &mse_fwd, "fused MSE loss", py::arg("pred"),
         py::arg("target"), py::arg("want_value") = true);
   m.def("mse_bwd", &mse_bwd, "MSE grad");
+  m.def("dropout", &dropout,
+        "dropout by Philox4x32-10 of (seed, offset, element); its own "
+        "backward");
+  m.def("dropout_next", &dropout_next,
+        "the state of one draw; steps the given state on in place");
+  m.def("logprobs_fwd", &logprobs_fwd,
+        "token log-probs + row entropy + top-k; one read of logits");
+  m.def("logprobs_bwd", &logprobs_bwd,
+        "dlogits from the gradients of log-probs, entropy and top-k",
+        py::arg("logits"), py::arg("tokens"), py::arg("stat"),
+        py::arg("entropy"), py::arg("ids"), py::arg("g_logp") = py::none(),
+        py::arg("g_entropy") = py::none(), py::arg("g_top") = py::none(),
+        py::arg("ignore") = -100);
   m.def("fused_sgd", &fused_sgd, "single-launch SGD apply");
   m.def("fused_momentum", &fused_momentum, "single-launch momentum apply");
   m.def("fused_adam", &fused_adam, "single-launch Adam apply");

@@ -1,0 +1,665 @@
+// Log-probabilities of given tokens with the entropy of their rows and the
+// k best alternatives, and the gradient of all three.
+//
+//   m = max x      s = sum e^(x-m)      t = sum e^(x-m) (x-m)
+//   l = log s                           logp_c = (x_c - m) - l
+//   H = -sum p log p = l - t / s        (both terms are >= 0: no cancelling)
+//   dx_c = g_logp [c = token] + sum_j g_j [c = id_j]
+//          - p_c (g_logp + sum_j g_j) - g_H p_c (logp_c + H)
+//
+// m and l are kept apart: their sum in 32 bits would lose l beside a large
+// m (a row masked by the type's lowest value, far-off logits).
+//
+// Forward reads the logits once: every thread keeps its own (m, s, t), a
+// block joins them, and a row may be split over blocks that a second kernel
+// joins.  The alternatives need no second pass over the row: a thread's
+// maximum orders the threads, and with (value, lowest index) as the order
+// the k best elements of a block all lie with the k threads whose maxima are
+// largest, so only those k threads' elements are read again.
+//
+// All sums and statistics are fp32; outputs are fp32.
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include "vec.h"
+
+#define TOP_MAX 32
+
+// (m, s, t) of a set of elements.  An empty set, or one of -inf alone, has
+// s = t = 0.  NaN and +inf end up in s as NaN.
+struct Stat {
+  float m, s, t;
+};
+
+// The set moved to the larger maximum m.
+__device__ __forceinline__ Stat stat_at(Stat a, float m) {
+  if (a.m == m || a.m == -INFINITY) return {m, a.s, a.t};
+  const float d = a.m - m;
+  const float f = __expf(d);
+  return {m, a.s * f, (a.t + a.s * d) * f};
+}
+
+__device__ __forceinline__ Stat stat_join(Stat a, Stat b) {
+  const float m = fmaxf(a.m, b.m);
+  a = stat_at(a, m);
+  b = stat_at(b, m);
+  return {m, a.s + b.s, a.t + b.t};
+}
+
+// An element in the order of the alternatives: larger values first, equal
+// values (both zeros among them) by the lower index.  0 is no element; a
+// NaN is none either, since its row has no alternatives.
+__device__ __forceinline__ unsigned long order_key(float x, unsigned idx) {
+  if (x != x) return 0;
+  const unsigned b = __float_as_uint(x + 0.0f);
+  const unsigned o = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  return ((unsigned long)o << 32) | (0xFFFFFFFFu - idx);
+}
+
+__device__ __forceinline__ float key_value(unsigned long key) {
+  const unsigned o = (unsigned)(key >> 32);
+  return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
+}
+
+__device__ __forceinline__ long key_index(unsigned long key) {
+  return (long)(0xFFFFFFFFu - (unsigned)key);
+}
+
+__device__ __forceinline__ unsigned long key_max(unsigned long a,
+                                                 unsigned long b) {
+  return a > b ? a : b;
+}
+
+__device__ __forceinline__ unsigned long wave_key_max(unsigned long v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1)
+    v = key_max(v, __shfl_xor(v, off, WAVE));
+  return v;
+}
+
+// Labels are int64, or fp32 that hold whole numbers (the engine's labels).
+struct Tokens {
+  const long* i64;
+  const float* f32;
+  long ignore;
+};
+
+__device__ __forceinline__ long token_of(const Tokens& t, long row) {
+  return t.i64 ? t.i64[row] : (long)t.f32[row];
+}
+
+struct RowOut {
+  float* logp;
+  float* entropy;
+  float* stat;  // [M, 2]: m and log s
+  float* top;   // [M, k]
+  long* ids;    // [M, k]
+};
+
+// What a row says when it is not to be read.
+__device__ __forceinline__ void write_ignored(const RowOut& o, long row,
+                                              int k, int tid, int nt) {
+  if (tid == 0) {
+    o.logp[row] = 0.0f;
+    o.entropy[row] = 0.0f;
+    o.stat[2 * row] = 0.0f;
+    o.stat[2 * row + 1] = 0.0f;
+  }
+  for (int j = tid; j < k; j += nt) {
+    o.top[row * k + j] = 0.0f;
+    o.ids[row * k + j] = -1;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void write_stats(const RowOut& o, long row,
+                                            Stat a, const T* xr, long C,
+                                            long token) {
+  const float l = a.s == 0.0f ? 0.0f : logf(a.s);
+  float lp;
+  if (token < 0 || token >= C) {
+    lp = NAN;  // no such token
+  } else if (a.s == 0.0f) {
+    lp = -INFINITY;  // every token of the row is impossible
+  } else {
+    lp = ((float)xr[token] - a.m) - l;
+  }
+  o.logp[row] = lp;
+  o.entropy[row] = a.s == 0.0f ? 0.0f : l - a.t / a.s;
+  o.stat[2 * row] = a.m;
+  o.stat[2 * row + 1] = l;
+}
+
+__device__ __forceinline__ void write_top(const RowOut& o, long row, int k,
+                                          int j, unsigned long key, Stat a) {
+  const bool none = a.s != a.s;  // a NaN or +inf: no distribution
+  float lp = NAN;
+  long id = -1;
+  if (!none && key != 0) {
+    const float x = key_value(key);
+    lp = x == -INFINITY ? -INFINITY : (x - a.m) - logf(a.s);
+    id = key_index(key);
+  }
+  o.top[row * k + j] = lp;
+  o.ids[row * k + j] = id;
+}
+
+// One block per (row, split).  NT threads; thread t owns the vectors
+// t, t + NT, t + 2 NT ... of the split and, if it is the last thread, the
+// elements behind the last whole vector.
+template <typename T, int NT, int UNROLL, bool TOP>
+__global__ void __launch_bounds__(NT)
+    logprobs_fwd_kernel(const T* __restrict__ logits, long stride,
+                        Tokens tokens, RowOut out, float* __restrict__ pstat,
+                        unsigned long* __restrict__ pkeys, long C, int splits,
+                        long span, int k) {
+  constexpr int N = Vec<T>::N;
+  constexpr int CAP = 512;
+  __shared__ Stat wstat[NT / WAVE];
+  __shared__ __attribute__((aligned(16))) unsigned long keys[TOP ? NT : 2];
+  __shared__ unsigned long cand[TOP ? CAP : 1];
+  __shared__ int owners[TOP_MAX];
+  __shared__ int count;
+  __shared__ unsigned long bar;
+
+  const int tid = threadIdx.x;
+  const int lane = tid & (WAVE - 1), wave = tid / WAVE;
+  const long row = blockIdx.x / splits;
+  const int split = blockIdx.x % splits;
+  const long token = token_of(tokens, row);
+  if (token == tokens.ignore) {
+    if (splits == 1) write_ignored(out, row, k, tid, NT);
+    return;
+  }
+  const T* xr = logits + row * stride;
+  const long lo = split * span;
+  const long hi = lo + span < C ? lo + span : C;
+  const int vecs = (int)((hi - lo) / N);  // whole vectors
+  const int tail = (int)((hi - lo) % N);
+
+  // -- one pass: (m, s, t) and where m came from
+  Stat a = {-INFINITY, 0.0f, 0.0f};
+  int from = tid;  // the vector, of this thread's, that raised m last
+  for (int v0 = tid; v0 < vecs; v0 += NT * UNROLL) {
+    typename Vec<T>::V v[UNROLL];
+    float x[UNROLL][N];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (v0 + u * NT < vecs)
+        v[u] = Vec<T>::load(xr + lo + (long)(v0 + u * NT) * N);
+    float gm = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const bool in = v0 + u * NT < vecs;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        x[u][j] = in ? (float)v[u][j] : -INFINITY;
+        gm = fmaxf(gm, x[u][j]);
+      }
+    }
+    if (gm > a.m) {
+      a = stat_at(a, gm);
+      if (TOP) from = v0;
+    }
+    if (a.m == -INFINITY) {
+      // nothing but -inf so far, and perhaps NaN
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (x[u][j] != x[u][j]) a.s = x[u][j];
+      continue;
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float d = x[u][j] - a.m;
+        const float e = __expf(d);
+        a.s += e;
+        // -inf: e is 0 and must meet a finite factor
+        a.t = fmaf(e, fmaxf(d, -1000.0f), a.t);
+      }
+  }
+  bool from_tail = false;
+  if (tid == NT - 1) {
+    for (int j = 0; j < tail; ++j) {
+      const float x = (float)xr[lo + (long)vecs * N + j];
+      if (x > a.m) {
+        a = stat_at(a, x);
+        from_tail = true;
+      }
+      if (a.m == -INFINITY) {
+        if (x != x) a.s = x;
+        continue;
+      }
+      const float d = x - a.m;
+      const float e = __expf(d);
+      a.s += e;
+      a.t = fmaf(e, fmaxf(d, -1000.0f), a.t);
+    }
+  }
+
+  // -- the block's (m, s, t)
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1)
+    a = stat_join(a, {__shfl_xor(a.m, off, WAVE), __shfl_xor(a.s, off, WAVE),
+                      __shfl_xor(a.t, off, WAVE)});
+  if (NT > WAVE) {
+    if (lane == 0) wstat[wave] = a;
+    __syncthreads();
+    a = wstat[0];
+#pragma unroll
+    for (int w = 1; w < NT / WAVE; ++w) a = stat_join(a, wstat[w]);
+  }
+  if (tid == 0) {
+    if (splits == 1) {
+      write_stats(out, row, a, xr, C, token);
+    } else {
+      float* p = pstat + ((long)row * splits + split) * 3;
+      p[0] = a.m;
+      p[1] = a.s;
+      p[2] = a.t;
+    }
+  }
+  if (!TOP) return;
+
+  // -- the thread's own best element, by reading its vectors again
+  unsigned long best = 0;
+  if (tid < vecs) {
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int at = from + u * NT;
+      if (at >= vecs) break;
+      const typename Vec<T>::V v = Vec<T>::load(xr + lo + (long)at * N);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        best = key_max(best,
+                       order_key((float)v[j], (unsigned)(lo + (long)at * N + j)));
+    }
+  }
+  if (tid == NT - 1 && (from_tail || tid >= vecs)) {
+    for (int j = 0; j < tail; ++j)
+      best = key_max(best, order_key((float)xr[lo + (long)vecs * N + j],
+                                     (unsigned)(lo + (long)vecs * N + j)));
+  }
+  keys[tid] = best;
+  if (tid == 0) {
+    count = 0;
+    bar = 0;
+  }
+  __syncthreads();
+  int rank = 0;
+  for (int i = 0; i < NT; ++i) rank += keys[i] > best ? 1 : 0;
+  if (best != 0 && rank < k) {
+    owners[rank] = tid;
+    atomicAdd(&count, 1);
+    if (rank == k - 1) bar = best;
+  }
+  __syncthreads();
+  const int nown = count;  // threads that own anything, at most k
+  const unsigned long floor_key = bar;
+  __syncthreads();
+  if (tid == 0) count = 0;
+  __syncthreads();
+
+  // -- the elements of those threads that reach the k-th best maximum
+  const int per = (vecs + NT - 1) / NT;  // vectors of one thread, at most
+  for (int w = tid; w < nown * per; w += NT) {
+    const int at = owners[w / per] + (w % per) * NT;
+    if (at >= vecs) continue;
+    const typename Vec<T>::V v = Vec<T>::load(xr + lo + (long)at * N);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const unsigned long key =
+          order_key((float)v[j], (unsigned)(lo + (long)at * N + j));
+      if (key != 0 && key >= floor_key) {
+        const int i = atomicAdd(&count, 1);
+        if (i < CAP) cand[i] = key;
+      }
+    }
+  }
+  for (int j = tid; j < tail; j += NT) {
+    const unsigned long key = order_key((float)xr[lo + (long)vecs * N + j],
+                                        (unsigned)(lo + (long)vecs * N + j));
+    if (key != 0 && key >= floor_key) {
+      const int i = atomicAdd(&count, 1);
+      if (i < CAP) cand[i] = key;
+    }
+  }
+  __syncthreads();
+  const int n = count;
+  unsigned long* pk =
+      splits == 1 ? nullptr : pkeys + ((long)row * splits + split) * k;
+  auto emit = [&](int j, unsigned long key) {
+    if (splits == 1)
+      write_top(out, row, k, j, key, a);
+    else
+      pk[j] = key;
+  };
+  if (n <= CAP) {
+    for (int i = tid; i < n; i += NT) {
+      const unsigned long key = cand[i];
+      int r = 0;
+      for (int j = 0; j < n; ++j) r += cand[j] > key ? 1 : 0;
+      if (r < k) emit(r, key);
+    }
+    for (int j = n + tid; j < k; j += NT) emit(j, 0);
+    return;
+  }
+  // More candidates than the list holds: large values that sit together in
+  // few threads' vectors.  Take them one after another, the largest below
+  // the last.
+  unsigned long last = ~0ul;
+  for (int j = 0; j < k; ++j) {
+    unsigned long top = 0;
+    for (int w = tid; w < nown * per; w += NT) {
+      const int at = owners[w / per] + (w % per) * NT;
+      if (at >= vecs) continue;
+      const typename Vec<T>::V v = Vec<T>::load(xr + lo + (long)at * N);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const unsigned long key =
+            order_key((float)v[i], (unsigned)(lo + (long)at * N + i));
+        if (key < last) top = key_max(top, key);
+      }
+    }
+    for (int i = tid; i < tail; i += NT) {
+      const unsigned long key = order_key((float)xr[lo + (long)vecs * N + i],
+                                          (unsigned)(lo + (long)vecs * N + i));
+      if (key < last) top = key_max(top, key);
+    }
+    top = wave_key_max(top);
+    __syncthreads();  // the list, or the last round's maxima, were read
+    if (lane == 0) cand[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NT / WAVE; ++w) top = key_max(top, cand[w]);
+    if (tid == 0) emit(j, top);
+    last = top;
+  }
+}
+
+// Joins the splits of a row, one wave a row.  Lane l holds split l.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    logprobs_join_kernel(const T* __restrict__ logits, long stride,
+                         Tokens tokens, RowOut out,
+                         const float* __restrict__ pstat,
+                         const unsigned long* __restrict__ pkeys, long M,
+                         long C, int splits, int k) {
+  const long row = (long)blockIdx.x * (256 / WAVE) + threadIdx.x / WAVE;
+  const int lane = threadIdx.x & (WAVE - 1);
+  if (row >= M) return;
+  const long token = token_of(tokens, row);
+  if (token == tokens.ignore) {
+    write_ignored(out, row, k, lane, WAVE);
+    return;
+  }
+  Stat a = {-INFINITY, 0.0f, 0.0f};
+  if (lane < splits) {
+    const float* p = pstat + (row * splits + lane) * 3;
+    a = {p[0], p[1], p[2]};
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1)
+    a = stat_join(a, {__shfl_xor(a.m, off, WAVE), __shfl_xor(a.s, off, WAVE),
+                      __shfl_xor(a.t, off, WAVE)});
+  if (lane == 0) write_stats(out, row, a, logits + row * stride, C, token);
+  // every split's list is sorted: take the largest head k times
+  const unsigned long* list = pkeys + (row * splits + lane) * k;
+  int at = 0;
+  unsigned long head = lane < splits && k > 0 ? list[0] : 0;
+  for (int j = 0; j < k; ++j) {
+    const unsigned long top = wave_key_max(head);
+    if (lane == 0) write_top(out, row, k, j, top, a);
+    if (top != 0 && head == top) {
+      ++at;
+      head = at < k ? list[at] : 0;
+    }
+  }
+}
+
+struct RowGrad {
+  const float* logp;     // each may be null: no gradient from there
+  const float* entropy;
+  const float* top;
+};
+
+// One block per (row, span).  The few places that take a gradient of their
+// own (the token, the alternatives) are listed first; a vector without one
+// of them costs one comparison per listed place, and a span that holds none
+// costs nothing.
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT)
+    logprobs_bwd_kernel(const T* __restrict__ logits, long stride,
+                        Tokens tokens, const float* __restrict__ stat,
+                        const float* __restrict__ entropy,
+                        const long* __restrict__ ids, RowGrad grad,
+                        T* __restrict__ dx, long C, int spans, long span,
+                        int k) {
+  constexpr int N = Vec<T>::N;
+  __shared__ long place[TOP_MAX + 1];
+  __shared__ float add[TOP_MAX + 1];
+  __shared__ int count;
+  const int tid = threadIdx.x;
+  const long row = blockIdx.x / spans;
+  const long lo = (long)(blockIdx.x % spans) * span;
+  const long hi = lo + span < C ? lo + span : C;
+  const T* xr = logits + row * stride;
+  T* dr = dx + row * C;
+  const long token = token_of(tokens, row);
+  const long vecs = (hi - lo) / N;
+
+  if (token == tokens.ignore) {
+    typename Vec<T>::V zero;
+#pragma unroll
+    for (int j = 0; j < N; ++j) zero[j] = (T)0.0f;
+    for (long v = tid; v < vecs; v += NT) Vec<T>::store(dr + lo + v * N, zero);
+    for (long c = lo + vecs * N + tid; c < hi; c += NT) dr[c] = (T)0.0f;
+    return;
+  }
+  const float m = stat[2 * row], l = stat[2 * row + 1];
+  const float H = entropy[row];
+  const float gp = grad.logp ? grad.logp[row] : 0.0f;
+  const float gh = grad.entropy ? grad.entropy[row] : 0.0f;
+  float share = gp;
+  if (grad.top)
+    for (int j = 0; j < k; ++j) share += grad.top[row * k + j];
+  const bool bad = grad.logp && (token < 0 || token >= C);  // no such token
+  if (bad) share = NAN;
+  // a row of -inf alone is constant
+  const bool constant = m == -INFINITY && l == 0.0f && !bad;
+  if (tid < WAVE) {  // k + 1 <= 33 places, listed in their order
+    long c = -1;
+    float g = 0.0f;
+    if (tid < k && grad.top) {
+      c = ids[row * k + tid];
+      g = grad.top[row * k + tid];
+    } else if (tid == k) {
+      c = token;
+      g = gp;
+    }
+    const bool here = !constant && c >= lo && c < hi && g != 0.0f;
+    const unsigned long all = __ballot(here);
+    if (here) {
+      const int i = __popcll(all & ((1ul << tid) - 1));
+      place[i] = c;
+      add[i] = g;
+    }
+    if (tid == 0) count = __popcll(all);
+  }
+  __syncthreads();
+  const int n = count;
+  auto at = [&](float x) -> float {
+    if (constant) return 0.0f;
+    const float d = (x - m) - l;
+    const float p = __expf(d);
+    // -inf: p is 0 and must meet a finite factor
+    return -p * fmaf(gh, fmaxf(d, -1000.0f) + H, share);
+  };
+  for (long v = tid; v < vecs; v += NT) {
+    const long c0 = lo + v * N;
+    const typename Vec<T>::V in = Vec<T>::load(xr + c0);
+    float d[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) d[j] = at((float)in[j]);
+    for (int i = 0; i < n; ++i) {
+      const long p = place[i] - c0;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (p == j) d[j] += add[i];
+    }
+    typename Vec<T>::V o;
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] = (T)d[j];
+    Vec<T>::store(dr + c0, o);
+  }
+  for (long c = lo + vecs * N + tid; c < hi; c += NT) {
+    float d = at((float)xr[c]);
+    for (int i = 0; i < n; ++i)
+      if (place[i] == c) d += add[i];
+    dr[c] = (T)d;
+  }
+}
+
+static Tokens check_logits(const torch::Tensor& logits,
+                           const torch::Tensor& tokens, int64_t ignore) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.size(1) >= 1 &&
+                  (logits.size(1) == 1 || logits.stride(1) == 1) &&
+                  logits.size(1) < (1l << 31),
+              "logits must be [rows, classes] on GPU with classes side by "
+              "side");
+  TORCH_CHECK(tokens.device() == logits.device() && tokens.dim() == 1 &&
+                  tokens.is_contiguous() &&
+                  tokens.size(0) == logits.size(0) &&
+                  (tokens.scalar_type() == torch::kInt64 ||
+                   tokens.scalar_type() == torch::kFloat32),
+              "tokens must be contiguous int64 or fp32 [rows] beside logits");
+  const bool whole = tokens.scalar_type() == torch::kInt64;
+  return {whole ? tokens.data_ptr<int64_t>() : nullptr,
+          whole ? nullptr : tokens.data_ptr<float>(), ignore};
+}
+
+std::vector<torch::Tensor> logprobs_fwd(torch::Tensor logits,
+                                        torch::Tensor tokens, int64_t k,
+                                        int64_t ignore) {
+  const Tokens tok = check_logits(logits, tokens, ignore);
+  TORCH_CHECK(k >= 0 && k <= TOP_MAX && k <= logits.size(1),
+              "top_k must be 0 .. min(32, classes)");
+  const at::cuda::CUDAGuard guard(logits.device());
+  const long M = logits.size(0), C = logits.size(1);
+  const auto f32 = logits.options().dtype(torch::kFloat32);
+  const auto i64 = logits.options().dtype(torch::kInt64);
+  auto logp = torch::empty({M}, f32), entropy = torch::empty({M}, f32),
+       stat = torch::empty({M, 2}, f32), top = torch::empty({M, k}, f32);
+  auto ids = torch::empty({M, k}, i64);
+  if (M == 0) return {logp, entropy, stat, top, ids};
+  const RowOut out = {logp.data_ptr<float>(), entropy.data_ptr<float>(),
+                      stat.data_ptr<float>(), top.data_ptr<float>(),
+                      ids.data_ptr<int64_t>()};
+  auto stream = at::cuda::getCurrentCUDAStream();
+  for_dtype(logits.scalar_type(), "logits", [&](auto t) {
+    using T = decltype(t);
+    constexpr int N = Vec<T>::N;
+    // Split rows until the blocks fill the 256 CUs twice, in spans of
+    // 4096 elements at least.
+    long splits = 1;
+    if (M < 512) splits = std::min<long>(64, std::min((512 + M - 1) / M,
+                                                      (C + 4095) / 4096));
+    long span = (C + splits - 1) / splits;
+    span = (span + N - 1) / N * N;
+    splits = (C + span - 1) / span;
+    TORCH_CHECK(M * splits < (1l << 31), "logits: too many rows");
+    torch::Tensor pstat, pkeys;
+    if (splits > 1) {
+      pstat = torch::empty({M, splits, 3}, f32);
+      pkeys = torch::empty({M, splits, k}, i64);
+    }
+    float* ps = splits > 1 ? pstat.data_ptr<float>() : nullptr;
+    auto* pk = splits > 1
+                   ? reinterpret_cast<unsigned long*>(pkeys.data_ptr())
+                   : nullptr;
+    const T* x = ptr<T>(logits);
+    auto go = [&](auto kernel, int nt) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(M * splits)), dim3(nt), 0,
+                         stream, x, (long)logits.stride(0), tok, out, ps, pk,
+                         C, (int)splits, span, (int)k);
+    };
+    // One wave a row while a row gives a wave no more than 4 vectors a
+    // lane; more rows are in flight then and nothing waits at a barrier.
+    if (span <= 4 * WAVE * N) {
+      if (k)
+        go(logprobs_fwd_kernel<T, 64, 1, true>, 64);
+      else
+        go(logprobs_fwd_kernel<T, 64, 1, false>, 64);
+    } else if (k) {
+      go(logprobs_fwd_kernel<T, 256, 2, true>, 256);
+    } else {
+      go(logprobs_fwd_kernel<T, 256, 2, false>, 256);
+    }
+    LAUNCH_OK();
+    if (splits > 1) {
+      hipLaunchKernelGGL((logprobs_join_kernel<T>),
+                         dim3((unsigned)((M + 3) / 4)), dim3(256), 0, stream,
+                         x, (long)logits.stride(0), tok, out, ps, pk, M, C,
+                         (int)splits, (int)k);
+      LAUNCH_OK();
+    }
+  });
+  return {logp, entropy, stat, top, ids};
+}
+
+static const float* row_grad(const c10::optional<torch::Tensor>& g,
+                             const torch::Tensor& logits, long n) {
+  if (!g.has_value()) return nullptr;
+  TORCH_CHECK(g->device() == logits.device() && g->is_contiguous() &&
+                  g->scalar_type() == torch::kFloat32 && g->numel() == n,
+              "row gradients must be contiguous fp32 beside logits");
+  return g->data_ptr<float>();
+}
+
+torch::Tensor logprobs_bwd(torch::Tensor logits, torch::Tensor tokens,
+                           torch::Tensor stat, torch::Tensor entropy,
+                           torch::Tensor ids,
+                           c10::optional<torch::Tensor> g_logp,
+                           c10::optional<torch::Tensor> g_entropy,
+                           c10::optional<torch::Tensor> g_top,
+                           int64_t ignore) {
+  const Tokens tok = check_logits(logits, tokens, ignore);
+  const long M = logits.size(0), C = logits.size(1);
+  TORCH_CHECK(ids.device() == logits.device() && ids.is_contiguous() &&
+                  ids.scalar_type() == torch::kInt64 && ids.dim() == 2 &&
+                  ids.size(0) == M && ids.size(1) <= TOP_MAX,
+              "ids must be contiguous int64 [rows, k]");
+  const int k = (int)ids.size(1);
+  const float* pl = row_grad(stat, logits, 2 * M);
+  const float* pe = row_grad(entropy, logits, M);
+  const RowGrad grad = {row_grad(g_logp, logits, M),
+                        row_grad(g_entropy, logits, M),
+                        row_grad(g_top, logits, M * k)};
+  const at::cuda::CUDAGuard guard(logits.device());
+  auto dx = torch::empty({M, C}, logits.options());
+  if (M == 0) return dx;
+  auto stream = at::cuda::getCurrentCUDAStream();
+  for_dtype(logits.scalar_type(), "logits", [&](auto t) {
+    using T = decltype(t);
+    constexpr int N = Vec<T>::N;
+    auto go = [&](auto kernel, int nt, long span) {
+      const long spans = (C + span - 1) / span;
+      TORCH_CHECK(M * spans < (1l << 31), "logits: too many rows");
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(M * spans)), dim3(nt), 0,
+                         stream, ptr<T>(logits), (long)logits.stride(0), tok,
+                         pl, pe, ids.data_ptr<int64_t>(), grad, ptr<T>(dx),
+                         C, (int)spans, span, k);
+    };
+    if (C <= 4 * WAVE * N) {
+      go(logprobs_bwd_kernel<T, 64>, 64, 4 * WAVE * N);
+    } else {
+      go(logprobs_bwd_kernel<T, 256>, 256, 256 * N * 4);
+    }
+  });
+  LAUNCH_OK();
+  return dx;
+}

@@ -25,6 +25,8 @@ SOURCES = [
     HERE / "hip" / "conv_nhwc.hip",
     HERE / "hip" / "norm.hip",
     HERE / "hip" / "dist_session.hip",
+    HERE / "hip" / "dropout.hip",
+    HERE / "hip" / "logprobs.hip",
 ]
 
 # Packed fp32 instructions (v_pk_add/mul/fma_f32) stay out of every kernel:
