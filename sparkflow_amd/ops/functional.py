@@ -845,6 +845,188 @@ def token_logprobs(logits, tokens, top_k: int = 0,
                          ids.reshape(shape + (top_k,)))
 
 
+# -- low-rank adapters --------------------------------------------------------
+
+_RANK_MAX, _ADAPTERS_MAX = 128, 1024
+
+
+class AdapterGroups:
+    """The rows of a batch grouped by adapter, for every ``adapter_add`` on
+    the same rows (the layers of a model): see ``adapter_groups``."""
+
+    def __init__(self, ids, adapters: int):
+        self.adapters = adapters
+        self.shape = ids.shape
+        self.ids = ids.detach().reshape(-1).long().contiguous()
+        self.device = ids.device
+        self.plan = ops.hip.adapter_plan(self.ids, adapters) \
+            if ops.use_hip(ids) else None
+
+
+def adapter_groups(ids, adapters: int) -> AdapterGroups:
+    """Groups rows by adapter once, for several ``adapter_add``.
+
+    ids: whole numbers in an integer type, one a row.  0 .. adapters - 1
+    name an adapter, a negative number none.
+    """
+    if ids.dtype == torch.bool or ids.is_floating_point() \
+            or ids.is_complex():
+        raise ValueError("ids must be whole numbers in an integer type, "
+                         "got %s" % (ids.dtype,))
+    if not 1 <= adapters <= _ADAPTERS_MAX:
+        raise ValueError("adapters must be within 1 and %d, got %r"
+                         % (_ADAPTERS_MAX, adapters))
+    return AdapterGroups(ids, adapters)
+
+
+class _AdapterAdd(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, base, x, a, b, scales, scale, groups, act: int):
+        if ops.use_hip(x):
+            z = ops.hip.adapter_shrink(x, a, groups.plan, scales, scale,
+                                       True)
+            y = ops.hip.adapter_expand(base, z, b, groups.plan, act, True)
+        else:
+            z, y = _adapter_cpu(base, x, a, b, scales, scale, groups, act)
+        ctx.save_for_backward(x, a, b, z, scales,
+                              y if act != ACT_NONE else None)
+        ctx.conf = (scale, groups, act)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, a, b, z, scales, y = ctx.saved_tensors
+        scale, groups, act = ctx.conf
+        need_base, need_x, need_a, need_b = ctx.needs_input_grad[:4]
+        e, r, _ = a.shape
+        dy = dy.contiguous()
+        if not ops.use_hip(x):
+            grads = _adapter_grad_cpu(x, a, b, z, scales, y, dy, scale,
+                                      groups, act)
+            return tuple(g if need else None for g, need in zip(
+                grads, ctx.needs_input_grad)) + (None,) * 4
+        if act != ACT_NONE:
+            dy = ops.hip.adapter_act_bwd(y, dy, act)
+        dx = da = db = None
+        if need_x or need_a:
+            dz = ops.hip.adapter_shrink(dy, b, groups.plan, scales, scale,
+                                        False)
+        if need_x:
+            dx = ops.hip.adapter_expand(None, dz, a, groups.plan, ACT_NONE,
+                                        False)
+        if need_a:
+            da = ops.hip.adapter_outer(x, dz, groups.plan, e, r, True)
+        if need_b:
+            db = ops.hip.adapter_outer(dy, z, groups.plan, e, r, False)
+        return (dy if need_base else None, dx, da, db) + (None,) * 4
+
+
+def _adapter_rows(groups, scales, scale):
+    for e in range(groups.adapters):
+        rows = (groups.ids == e).nonzero().squeeze(1)
+        if len(rows):
+            yield e, rows, scale if scales is None else scales[e]
+
+
+def _adapter_cpu(base, x, a, b, scales, scale, groups, act):
+    f32 = torch.float32
+    y = base.to(f32).clone()
+    z = torch.zeros(x.shape[0], a.shape[1])
+    for e, rows, s in _adapter_rows(groups, scales, scale):
+        z[rows] = s * (x[rows].to(f32) @ a[e].to(f32).t())
+        y[rows] += z[rows] @ b[e].to(f32).t()
+    y[groups.ids >= groups.adapters] = float("nan")
+    return z, _act_fwd(y, act).to(base.dtype)
+
+
+def _adapter_grad_cpu(x, a, b, z, scales, y, dy, scale, groups, act):
+    f32 = torch.float32
+    if act != ACT_NONE:
+        dy = _act_bwd_from_out(y.to(f32), dy.to(f32), act).to(dy.dtype)
+    dx, da, db = (torch.zeros(t.shape) for t in (x, a, b))
+    for e, rows, s in _adapter_rows(groups, scales, scale):
+        g = dy[rows].to(f32)
+        dz = s * (g @ b[e].to(f32))
+        dx[rows] = dz @ a[e].to(f32)
+        da[e] = dz.t() @ x[rows].to(f32)
+        db[e] = g.t() @ z[rows]
+    dx[groups.ids >= groups.adapters] = float("nan")
+    return dy, dx.to(x.dtype), da.to(a.dtype), db.to(b.dtype)
+
+
+def adapter_add(base, x, a, b, ids, scale=1.0, act="none"):
+    """act(base + scale * (x A^T) B^T), each row through its own adapter:
+    low-rank adapters of many requests beside a shared projection.
+
+    base: [..., outputs], what the projection gave (before its activation);
+    x: [..., inputs], what it was given; both are read in place where their
+    last axis lies side by side.  a: [adapters, rank, inputs], b: [adapters,
+    outputs, rank], all in one type of fp32, bf16 or fp16; sums are 32 bits
+    wide and every result is rounded once.  rank is at most 128, adapters
+    1024.
+
+    ids: one whole number a row (the leading shape of x), or the
+    ``adapter_groups`` of them, which the layers of a model share.  A
+    negative id is a row without an adapter: act(base).  An id of
+    ``adapters`` or more cannot be refused without waiting for the device:
+    the row is NaN, and so is its gradient of x.
+
+    scale: a number, or fp32 [adapters].  Gradients flow to base, x, a and
+    b; an adapter that no row uses has a gradient of zero.
+    """
+    act = ACT_CODES[act] if isinstance(act, str) else act
+    tensors = (("base", base), ("x", x), ("a", a), ("b", b))
+    for name, t in tensors:
+        _check_float(name, t)
+        if t.dtype != x.dtype or t.device != x.device:
+            raise ValueError("%s is %s on %s and x %s on %s" % (
+                name, t.dtype, t.device, x.dtype, x.device))
+    if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] \
+            or a.shape[1] != b.shape[2]:
+        raise ValueError("a [adapters, rank, inputs] and b [adapters, "
+                         "outputs, rank] do not fit: %s and %s"
+                         % (tuple(a.shape), tuple(b.shape)))
+    e, r, k = a.shape
+    n = b.shape[1]
+    if not 1 <= r <= _RANK_MAX or k < 1 or n < 1:
+        raise ValueError("rank must be within 1 and %d, and inputs and "
+                         "outputs at least 1: %s and %s"
+                         % (_RANK_MAX, tuple(a.shape), tuple(b.shape)))
+    groups = ids if isinstance(ids, AdapterGroups) else None
+    lead = ids.shape
+    if x.shape != lead + (k,) or base.shape != lead + (n,):
+        raise ValueError("x %s and base %s do not fit ids %s and adapters "
+                         "of %d inputs and %d outputs" % (
+                             tuple(x.shape), tuple(base.shape), tuple(lead),
+                             k, n))
+    if ids.device != x.device:
+        raise ValueError("x is on %s and ids on %s" % (x.device, ids.device))
+    scales = None
+    if isinstance(scale, torch.Tensor):
+        if scale.requires_grad:
+            raise ValueError("scale takes no gradient: detach it")
+        if scale.shape != (e,) or scale.dtype != torch.float32 \
+                or scale.device != x.device:
+            raise ValueError("scale must be a number, or fp32 [%d] beside x"
+                             % e)
+        scales, scale = scale.contiguous(), 1.0
+    if groups is None:
+        groups = adapter_groups(ids, e)
+    elif groups.adapters != e:
+        raise ValueError("ids were grouped for %d adapters, not %d"
+                         % (groups.adapters, e))
+
+    def rows(t, width):
+        t = t.reshape(-1, width)
+        return t if t.stride(1) == 1 or width == 1 else t.contiguous()
+
+    y = _AdapterAdd.apply(rows(base, n), rows(x, k), a.contiguous(),
+                          b.contiguous(), scales, float(scale), groups, act)
+    return y.reshape(base.shape)
+
+
 def argmax_rows(y: torch.Tensor) -> torch.Tensor:
     """Rowwise argmax prediction head (reference tf.argmax(out, 1))."""
     if ops.use_hip(y):

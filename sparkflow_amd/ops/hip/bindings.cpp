@@ -63,6 +63,21 @@ torch::Tensor logprobs_bwd(torch::Tensor logits, torch::Tensor tokens,
                            c10::optional<torch::Tensor> g_top,
                            int64_t ignore);
 
+// adapter.hip — low-rank adapters of many requests
+torch::Tensor adapter_plan(torch::Tensor ids, int64_t E);
+torch::Tensor adapter_shrink(torch::Tensor x, torch::Tensor w,
+                             torch::Tensor plan,
+                             c10::optional<torch::Tensor> scales,
+                             double scale, bool kmajor);
+torch::Tensor adapter_expand(c10::optional<torch::Tensor> base,
+                             torch::Tensor z, torch::Tensor w,
+                             torch::Tensor plan, int64_t act, bool rmajor);
+torch::Tensor adapter_outer(torch::Tensor x, torch::Tensor z,
+                            torch::Tensor plan, int64_t E, int64_t R,
+                            bool kmajor);
+torch::Tensor adapter_act_bwd(torch::Tensor y, torch::Tensor dy,
+                              int64_t act);
+
 // optim.hip
 void fused_sgd(torch::Tensor p, torch::Tensor g, double lr);
 void fused_momentum(torch::Tensor p, torch::Tensor g, torch::Tensor acc,
@@ -213,6 +228,19 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("entropy"), py::arg("ids"), py::arg("g_logp") = py::none(),
         py::arg("g_entropy") = py::none(), py::arg("g_top") = py::none(),
         py::arg("ignore") = -100);
+  m.def("adapter_plan", &adapter_plan,
+        "rows grouped by adapter: order, groups and tiles of 16 rows");
+  m.def("adapter_shrink", &adapter_shrink,
+        "z = scale * x w^T by adapter, fp32, in grouped order",
+        py::arg("x"), py::arg("w"), py::arg("plan"), py::arg("scales"),
+        py::arg("scale"), py::arg("kmajor"));
+  m.def("adapter_expand", &adapter_expand,
+        "act(base + z w^T) by adapter", py::arg("base"), py::arg("z"),
+        py::arg("w"), py::arg("plan"), py::arg("act"), py::arg("rmajor"));
+  m.def("adapter_outer", &adapter_outer,
+        "sums of z^T x over each adapter's rows");
+  m.def("adapter_act_bwd", &adapter_act_bwd,
+        "activation backward from output, fp32 / bf16 / fp16");
   m.def("fused_sgd", &fused_sgd, "single-launch SGD apply");
   m.def("fused_momentum", &fused_momentum, "single-launch momentum apply");
   m.def("fused_adam", &fused_adam, "single-launch Adam apply");

@@ -27,6 +27,7 @@ SOURCES = [
     HERE / "hip" / "dist_session.hip",
     HERE / "hip" / "dropout.hip",
     HERE / "hip" / "logprobs.hip",
+    HERE / "hip" / "adapter.hip",
 ]
 
 # Packed fp32 instructions (v_pk_add/mul/fma_f32) stay out of every kernel:

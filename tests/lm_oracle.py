@@ -134,3 +134,61 @@ def logprobs_tol(want, entropy, c):
                        torch.zeros_like(want))
     n = sum_error(c) * (1 + (math.log(c + 1) if entropy else 0))
     return (2 * n + 8 + 8 * size + 2 * math.log(c + 1)) * U32
+
+
+# -- low-rank adapters --------------------------------------------------------
+
+
+def depth(n):
+    """Additions that one of n terms goes through at most: sums are split
+    over four waves at least, and 40 covers the steps that join them."""
+    return n / 4 + 40
+
+
+def adapter(base, x, a, b, ids, scale, g=None):
+    """y (and dx, da, db for the gradient g of y) by adapter in 64 bits,
+    each with the bound of a computation that sums in 32 bits and rounds
+    once to the inputs' type."""
+    dtype = x.dtype
+    base, x, a, b = (t.detach().cpu().double() for t in (base, x, a, b))
+    ids = ids.cpu()
+    e, r, k = a.shape
+    n, m = b.shape[1], x.shape[0]
+    y, dx = base.clone(), torch.zeros_like(x)
+    ty, tx = base.abs() * 2 * U32, torch.zeros_like(x)
+    da, db = torch.zeros_like(a), torch.zeros_like(b)
+    ta, tb = torch.zeros_like(a), torch.zeros_like(b)
+    for i in range(e):
+        at = (ids == i).nonzero().squeeze(1)
+        if not len(at):
+            continue
+        s = float(scale[i]) if isinstance(scale, torch.Tensor) else scale
+        s_err = 2 * U32  # the scale in 32 bits, and its product
+        xa, ba = x[at], b[i].abs()
+        z = s * (xa @ a[i].T)
+        z_size = abs(s) * (xa.abs() @ a[i].abs().T)
+        z_err = z_size * (depth(k) * U32 + s_err)
+        y[at] += z @ b[i].T
+        ty[at] += z_err @ ba.T + (z.abs() + z_err) @ ba.T * (r + 4) * U32
+        if g is None:
+            continue
+        ga = g[at].detach().cpu().double()
+        dz = s * (ga @ b[i])
+        dz_err = abs(s) * (ga.abs() @ ba) * (depth(n) * U32 + s_err)
+        dx[at] = dz @ a[i]
+        tx[at] = dz_err @ a[i].abs() + (
+            (dz.abs() + dz_err) @ a[i].abs()) * (r + 4) * U32
+        da[i], db[i] = dz.T @ xa, ga.T @ z
+        d = depth(len(at)) * U32
+        ta[i] = dz_err.T @ xa.abs() + (dz.abs() + dz_err).T @ xa.abs() * d
+        tb[i] = ga.abs().T @ z_err + ga.abs().T @ (z.abs() + z_err) * d
+
+    def rounded(t, tol):
+        tol = tol + (t.abs() + tol) * half_step(dtype) + 1e-37
+        return tol + (2.0 ** -25 if dtype == torch.float16 else 0)
+
+    out = [(y, rounded(y, ty))]
+    if g is not None:
+        out += [(dx, rounded(dx, tx)), (da, rounded(da, ta)),
+                (db, rounded(db, tb))]
+    return out

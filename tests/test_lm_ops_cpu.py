@@ -179,3 +179,113 @@ def test_logprobs_refuses():
                                create_graph=True)
     with pytest.raises(RuntimeError):  # no second derivative
         g.sum().backward()
+
+
+# -- low-rank adapters --------------------------------------------------------
+
+
+def _adapter_inputs(m, k, n, r, e, dtype=torch.float32, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+
+    def normal(*shape, std=1.0):
+        return (torch.randn(*shape, generator=gen) * std).to(dtype)
+
+    return (normal(m, n), normal(m, k), normal(e, r, k, std=k ** -0.5),
+            normal(e, n, r, std=r ** -0.5),
+            torch.randint(-1, e, (m,), generator=gen),
+            torch.rand(e, generator=gen) + 0.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 1, 1, 1, 1), (9, 20, 7, 3, 4),
+                                   (40, 17, 33, 16, 2), (5, 8, 8, 2, 30)])
+def test_adapter_add(dtype, shape):
+    base, x, a, b, ids, scale = _adapter_inputs(*shape, dtype=dtype)
+    leaves = [t.clone().requires_grad_() for t in (base, x, a, b)]
+    y = F.adapter_add(*leaves, ids, scale=scale)
+    g = torch.randn(y.shape).to(dtype)
+    grads = torch.autograd.grad(y, leaves, g)
+    assert torch.equal(grads[0], g)
+    want = oracle.adapter(base, x, a, b, ids, scale, g)
+    for got, (value, tol) in zip((y,) + grads[1:], want):
+        assert got.dtype == dtype
+        assert ((got.detach().double() - value).abs() <= tol).all()
+
+
+def test_adapter_add_scale_act_groups_and_shapes():
+    base, x, a, b, ids, _ = _adapter_inputs(12, 6, 5, 2, 3)
+    y = F.adapter_add(base, x, a, b, ids, scale=0.5)
+    value, tol = oracle.adapter(base, x, a, b, ids, 0.5)[0]
+    assert ((y.double() - value).abs() <= tol).all()
+    relu = F.adapter_add(base, x, a, b, ids, scale=0.5, act="relu")
+    assert torch.equal(relu, torch.relu(y))
+    groups = F.adapter_groups(ids, 3)
+    assert torch.equal(F.adapter_add(base, x, a, b, groups, scale=0.5), y)
+    shaped = F.adapter_add(base.reshape(3, 4, 5), x.reshape(3, 4, 6), a, b,
+                           ids.reshape(3, 4), scale=0.5)
+    assert torch.equal(shaped.reshape(12, 5), y)
+    none = F.adapter_add(base, x, a, b, torch.full_like(ids, -7))
+    assert torch.equal(none, base)
+    bad = ids.clone()
+    bad[3] = 3
+    y = F.adapter_add(base, x, a, b, bad)
+    assert torch.isnan(y[3]).all() and torch.isfinite(y[:3]).all()
+
+
+def test_adapter_add_act_gradient_by_differences():
+    base, x, a, b, ids, scale = _adapter_inputs(6, 5, 4, 2, 2, seed=3)
+    ids[0], ids[1] = 0, -1
+    leaves = [t.clone().requires_grad_() for t in (base, x, a, b)]
+    g = torch.randn(6, 4)
+    y = F.adapter_add(*leaves, ids, scale=scale, act="sigmoid")
+    grads = torch.autograd.grad(y, leaves, g)
+
+    def loss(*ts):
+        pre = oracle.adapter(*ts, ids, scale)[0][0]
+        return float((torch.sigmoid(pre) * g).sum())
+
+    for w in range(4):
+        ts = [t.double() for t in (base, x, a, b)]
+        for i in range(ts[w].numel()):
+            up, down = (list(ts), list(ts))
+            up[w], down[w] = ts[w].clone(), ts[w].clone()
+            up[w].view(-1)[i] += 1e-5
+            down[w].view(-1)[i] -= 1e-5
+            slope = (loss(*up) - loss(*down)) / 2e-5
+            assert abs(float(grads[w].reshape(-1)[i]) - slope) < 1e-5
+
+
+def test_adapter_add_refuses():
+    base, x, a, b, ids, scale = _adapter_inputs(4, 6, 5, 2, 3)
+
+    def refused(match, **changed):
+        args = dict(base=base, x=x, a=a, b=b, ids=ids)
+        args.update(changed)
+        with pytest.raises(ValueError, match=match):
+            F.adapter_add(**args)
+
+    refused("fp32, bf16 or fp16", base=base.double())
+    refused("base is torch.float16", base=base.half())
+    refused("b is torch.bfloat16", b=b.bfloat16())
+    refused("do not fit", a=a[:2])
+    refused("do not fit", b=b[:, :, :1])
+    refused("do not fit", a=a[0])
+    refused("x .* do not fit", x=x[:, :5])
+    refused("x .* do not fit", base=base[:3])
+    refused("x .* do not fit", ids=ids[:3])
+    refused("integer type", ids=ids.float())
+    refused("integer type", ids=ids > 0)
+    refused("ids on meta", ids=ids.to("meta"))
+    refused("scale must", scale=scale[:2])
+    refused("scale must", scale=scale.double())
+    refused("no gradient", scale=scale.clone().requires_grad_())
+    refused("grouped for 4", ids=F.adapter_groups(ids, 4))
+    refused("rank must", a=torch.randn(3, 129, 6), b=torch.randn(3, 5, 129))
+    refused("rank must", a=a[:, :0], b=b[:, :, :0])
+    refused("within 1 and 1024", a=torch.randn(1025, 1, 6),
+            b=torch.randn(1025, 5, 1))
+    for e in (0, 1025):
+        with pytest.raises(ValueError, match="adapters must be"):
+            F.adapter_groups(ids, e)
+    with pytest.raises(KeyError):
+        F.adapter_add(base, x, a, b, ids, act="tanh")

@@ -421,3 +421,259 @@ def test_logprobs_captured():
         torch.cuda.synchronize()
         for a, b in zip(held, step()):
             assert torch.equal(a, b)
+
+
+# -- low-rank adapters --------------------------------------------------------
+
+
+def _adapter_inputs(m, k, n, r, e, dtype=torch.float32, seed=0):
+    gen = torch.Generator().manual_seed(seed + 100)
+    ids = torch.randint(-1, e, (m,), generator=gen).to(DEV)
+    scale = (torch.rand(e, generator=gen) + 0.5).to(DEV)
+    return (_randn(m, n, dtype=dtype, seed=seed),
+            _randn(m, k, dtype=dtype, seed=seed + 1),
+            _randn(e, r, k, dtype=dtype, seed=seed + 2, std=k ** -0.5),
+            _randn(e, n, r, dtype=dtype, seed=seed + 3, std=r ** -0.5),
+            ids, scale)
+
+
+def _check_adapter(base, x, a, b, ids, scale, seed=50):
+    leaves = [t.detach().requires_grad_() for t in (base, x, a, b)]
+    y = F.adapter_add(*leaves, ids, scale=scale)
+    g = _randn(*y.shape, dtype=x.dtype, seed=seed)
+    grads = torch.autograd.grad(y, leaves, g)
+    assert torch.equal(grads[0], g)
+    want = oracle.adapter(base, x, a, b, ids, scale, g)
+    for got, (value, tol) in zip((y,) + grads[1:], want):
+        assert got.dtype == x.dtype and got.is_contiguous()
+        _within(got, value, tol)
+    return y, grads
+
+
+@pytest.mark.parametrize("m,e", [(0, 1), (1, 1), (5, 3), (16, 2), (17, 1),
+                                 (300, 4), (1000, 1024), (4097, 5)])
+def test_adapter_plan(m, e):
+    gen = torch.Generator().manual_seed(m)
+    ids = torch.randint(-2, e + 2, (m,), generator=gen)
+    plan = ops.hip.adapter_plan(ids.to(DEV), e).cpu()
+    group = torch.where(ids < 0, e, torch.where(ids >= e, e + 1, ids))
+    order = torch.sort(group, stable=True)[1]
+    assert torch.equal(plan[:m].long(), order)
+    counts = torch.bincount(group, minlength=e + 2)
+    seg, tbase = plan[m:m + e + 3], plan[m + e + 3:m + 2 * e + 6]
+    assert seg.tolist() == [0] + counts.cumsum(0).tolist()
+    tiles = (counts + 15) // 16
+    assert tbase.tolist() == [0] + tiles.cumsum(0).tolist()
+    most = m // 16 + min(e + 2, m)
+    of, place = plan[m + 2 * e + 6:].reshape(2, most)
+    n = int(tiles.sum())
+    want = [(g, int(seg[g]) + 16 * j) for g in range(e + 2)
+            for j in range(int(tiles[g]))]
+    assert list(zip(of[:n].tolist(), place[:n].tolist())) == want
+    assert (of[n:] == -1).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [
+    # rows, inputs, outputs, rank, adapters
+    (1, 1, 1, 1, 1), (1, 64, 64, 16, 4), (3, 8, 8, 2, 2), (16, 32, 32, 16, 1),
+    (17, 33, 65, 7, 3), (32, 512, 384, 16, 64), (33, 100, 31, 17, 2),
+    (50, 257, 129, 33, 5), (64, 96, 200, 64, 3), (70, 130, 70, 65, 2),
+    (40, 64, 48, 128, 2), (300, 784, 256, 8, 4), (777, 1000, 513, 12, 17),
+    (1025, 40, 24, 5, 3), (2500, 200, 136, 20, 3), (1500, 64, 72, 100, 40)])
+def test_adapter_values(dtype, shape):
+    _check_adapter(*_adapter_inputs(*shape, dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m", [60, 2000])
+@pytest.mark.parametrize("ids", ["none", "one", "last", "runs", "absent"])
+def test_adapter_orders(dtype, m, ids):
+    base, x, a, b, _, scale = _adapter_inputs(m, 72, 50, 9, 6, dtype=dtype)
+    at = torch.arange(m, device=DEV)
+    chosen = {"none": torch.full_like(at, -1), "one": torch.zeros_like(at),
+              "last": torch.full_like(at, 5), "runs": at * 7 // m - 1,
+              "absent": at % 2 * 3}[ids]
+    y, grads = _check_adapter(base, x, a, b, chosen, scale)
+    for e in range(6):
+        if not (chosen == e).any():
+            assert (grads[2][e] == 0).all() and (grads[3][e] == 0).all()
+    if ids == "none":
+        assert torch.equal(y, base) and (grads[1] == 0).all()
+
+
+def test_adapter_unknown_ids_give_nan():
+    for act in ("none", "relu", "sigmoid"):
+        base, x, a, b, ids, scale = _adapter_inputs(40, 30, 20, 4, 3)
+        bad = ids.clone()
+        bad[7], bad[30] = 3, 2 ** 40
+        x.requires_grad_()
+        y = F.adapter_add(base, x, a, b, bad, scale=scale, act=act)
+        (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+        ok = torch.ones(40, dtype=torch.bool, device=DEV)
+        ok[[7, 30]] = False
+        assert torch.isnan(y[~ok]).all() and torch.isnan(dx[~ok]).all()
+        want = F.adapter_add(base, x, a, b, ids, scale=scale, act=act)
+        assert torch.equal(y[ok], want[ok])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ["relu", "sigmoid"])
+def test_adapter_act(dtype, act):
+    base, x, a, b, ids, scale = _adapter_inputs(200, 90, 77, 6, 4,
+                                                dtype=dtype)
+    leaves = [t.requires_grad_() for t in (base, x, a, b)]
+    y = F.adapter_add(*leaves, ids, scale=0.25, act=act)
+    g = _randn(200, 77, dtype=dtype, seed=9)
+    grads = torch.autograd.grad(y, leaves, g)
+    pre, tol = oracle.adapter(base, x, a, b, ids, 0.25)[0]
+    fn = torch.relu if act == "relu" else torch.sigmoid
+    # neither has a slope above 1, so pre's error is not enlarged; __expf
+    # and the division are within 8 half steps of 32 bits.  What is rounded
+    # to the type is fn(pre), by half a step of fn(pre): near pre = 0 a
+    # sigmoid is 1/2, whose half step pre's own does not cover
+    _within(y, fn(pre), tol + 8 * oracle.U32
+            + fn(pre) * oracle.half_step(dtype) * 1.01)
+    out = y.detach()
+    slope = (out > 0).float() if act == "relu" else (
+        out.float() * (1 - out.float()))
+    d = (g.float() * slope).to(dtype)
+    _within(grads[0], d.double().cpu(), d.double().cpu().abs() * (
+        4 * oracle.U32 + 2 * oracle.half_step(dtype)) + 2.0 ** -24)
+    want = oracle.adapter(base, x, a, b, ids, 0.25, grads[0])
+    for got, (value, tol) in zip(grads[1:], want[1:]):
+        _within(got, value, tol)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_adapter_layouts(dtype):
+    base, x, a, b, ids, scale = _adapter_inputs(48, 65, 33, 5, 3,
+                                                dtype=dtype)
+    want = F.adapter_add(base, x, a, b, ids, scale=scale)
+    wide_x = torch.full((48, 100), math.nan, dtype=dtype, device=DEV)
+    wide_x[:, 3:68] = x
+    wide_base = torch.full((48, 50), math.nan, dtype=dtype, device=DEV)
+    wide_base[:, 1:34] = base
+    leaf = wide_x[:, 3:68].detach().requires_grad_()
+    got = F.adapter_add(wide_base[:, 1:34], leaf, a, b, ids, scale=scale)
+    assert torch.equal(got, want)
+    g = _randn(33, 48, dtype=dtype, seed=5).t()  # another order
+    (dx,) = torch.autograd.grad(got, leaf, g)
+    flat = x.clone().requires_grad_()
+    (dw,) = torch.autograd.grad(
+        F.adapter_add(base, flat, a, b, ids, scale=scale), flat,
+        g.contiguous())
+    assert torch.equal(dx, dw)
+    other = F.adapter_add(
+        base.t().contiguous().t(), x.t().contiguous().t(),
+        a.transpose(1, 2).contiguous().transpose(1, 2),
+        b.transpose(1, 2).contiguous().transpose(1, 2), ids.int(),
+        scale=scale)
+    assert torch.equal(other, want)
+    shaped = F.adapter_add(base.reshape(4, 12, 33), x.reshape(4, 12, 65), a,
+                           b, ids.reshape(4, 12), scale=scale)
+    assert torch.equal(shaped.reshape(48, 33), want)
+    # one adapter for all, given once and broadcast: its gradient is summed
+    one = a[:1].detach().requires_grad_()
+    y = F.adapter_add(base, x, one.expand(3, 5, 65), b, ids, scale=scale)
+    (da,) = torch.autograd.grad(y, one, g.contiguous())
+    each = a[:1].detach().repeat(3, 1, 1).requires_grad_()
+    y = F.adapter_add(base, x, each, b, ids, scale=scale)
+    (de,) = torch.autograd.grad(y, each, g.contiguous())
+    torch.testing.assert_close(da, de.sum(0, keepdim=True))
+
+
+def test_adapter_partial_gradients_and_groups():
+    base, x, a, b, ids, scale = _adapter_inputs(90, 40, 30, 4, 3)
+    g = _randn(90, 30, seed=6)
+    full = [t.detach().requires_grad_() for t in (base, x, a, b)]
+    groups = F.adapter_groups(ids, 3)
+    y = F.adapter_add(*full, groups, scale=scale)
+    every = torch.autograd.grad(y, full, g)
+    for i in range(4):
+        ts = [t.detach().clone() for t in (base, x, a, b)]
+        ts[i].requires_grad_()
+        y = F.adapter_add(*ts, ids, scale=scale)
+        (one,) = torch.autograd.grad(y, ts[i], g)
+        assert torch.equal(one, every[i])
+
+
+def test_adapter_broken_row_stays_alone():
+    base, x, a, b, ids, scale = _adapter_inputs(64, 96, 40, 16, 2)
+    ids = torch.arange(64, device=DEV) % 2
+    want = F.adapter_add(base, x, a, b, ids, scale=scale)
+    x[10, 5] = math.nan
+    x[11, 5] = math.inf
+    y = F.adapter_add(base, x, a, b, ids, scale=scale)
+    ok = torch.ones(64, dtype=torch.bool, device=DEV)
+    ok[10:12] = False
+    assert torch.equal(y[ok], want[ok])
+    assert not torch.isfinite(y[10:12]).any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_adapter_small_numbers(dtype):
+    """Subnormal inputs of the type are not flushed."""
+    tiny = torch.finfo(dtype).smallest_normal / 4
+    k = 64
+    x = torch.full((16, k), tiny, dtype=dtype, device=DEV)
+    a = torch.full((1, 4, k), 2.0 ** 13, dtype=dtype, device=DEV)
+    b = torch.full((1, 8, 4), 2.0 ** 10, dtype=dtype, device=DEV)
+    base = torch.zeros(16, 8, dtype=dtype, device=DEV)
+    ids = torch.zeros(16, dtype=torch.int64, device=DEV)
+    want = float(x[0, 0]) * k * 2.0 ** 13 * 4 * 2.0 ** 10
+    y = F.adapter_add(base, x, a, b, ids)
+    assert float(x[0, 0]) > 0 or dtype == torch.float32
+    torch.testing.assert_close(y.double(), torch.full_like(y, 1).double()
+                               * want, rtol=1e-2, atol=0)
+
+
+def test_adapter_offsets_past_32_bits():
+    m, k, n = 300001, 8192, 24
+    x = torch.empty(m, k, dtype=torch.bfloat16, device=DEV)
+    x.normal_(generator=torch.Generator(DEV).manual_seed(2))
+    base, _, a, b, _, scale = _adapter_inputs(8, k, n, 16, 3,
+                                              dtype=torch.bfloat16)
+    base = base.repeat(m // 8 + 1, 1)[:m].contiguous()
+    ids = torch.arange(m, device=DEV) % 4 - 1
+    leaf = x.requires_grad_()
+    y = F.adapter_add(base, leaf, a, b, ids, scale=scale)
+    g = _randn(8, n, dtype=torch.bfloat16, seed=3).repeat(m // 8 + 1, 1)[:m]
+    (dx,) = torch.autograd.grad(y, leaf, g)
+    pick = torch.tensor([0, 1, 262144, 262145, 262147, m - 2, m - 1],
+                        device=DEV)
+    want = oracle.adapter(base[pick], x[pick], a, b, ids[pick], scale,
+                          g[pick])
+    _within(y[pick], *want[0])
+    _within(dx[pick], *want[1])
+
+
+def test_adapter_captured_and_streams():
+    base, x, a, b, ids, scale = _adapter_inputs(
+        130, 256, 192, 16, 7, dtype=torch.bfloat16)
+    leaves = [t.clone().requires_grad_() for t in (base, x, a, b)]
+    g = _randn(130, 192, dtype=torch.bfloat16, seed=8)
+    ids = ids.clone()
+
+    def step():
+        y = F.adapter_add(*leaves, ids, scale=scale)
+        return (y.detach(),) + torch.autograd.grad(y, leaves, g)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        on_side = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for p, q in zip(on_side, step()):
+        assert torch.equal(p, q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(4):
+        with torch.no_grad():
+            leaves[1].copy_(x * (1 + i))
+        ids.copy_((ids + 2) % 8 - 1)
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(held, step()):
+            assert torch.equal(p, q)
