@@ -884,9 +884,9 @@ class _AdapterAdd(torch.autograd.Function):
     @staticmethod
     def forward(ctx, base, x, a, b, scales, scale, groups, act: int):
         if ops.use_hip(x):
-            z = ops.hip.adapter_shrink(x, a, groups.plan, scales, scale,
+            z = ops.hip.adapter_shrink(x, a, groups.ids, groups.plan, scales, scale,
                                        True)
-            y = ops.hip.adapter_expand(base, z, b, groups.plan, act, True)
+            y = ops.hip.adapter_expand(base, z, b, groups.ids, groups.plan, act, True)
         else:
             z, y = _adapter_cpu(base, x, a, b, scales, scale, groups, act)
         ctx.save_for_backward(x, a, b, z, scales,
@@ -911,15 +911,15 @@ class _AdapterAdd(torch.autograd.Function):
             dy = ops.hip.adapter_act_bwd(y, dy, act)
         dx = da = db = None
         if need_x or need_a:
-            dz = ops.hip.adapter_shrink(dy, b, groups.plan, scales, scale,
+            dz = ops.hip.adapter_shrink(dy, b, groups.ids, groups.plan, scales, scale,
                                         False)
         if need_x:
-            dx = ops.hip.adapter_expand(None, dz, a, groups.plan, ACT_NONE,
+            dx = ops.hip.adapter_expand(None, dz, a, groups.ids, groups.plan, ACT_NONE,
                                         False)
         if need_a:
-            da = ops.hip.adapter_outer(x, dz, groups.plan, e, r, True)
+            da = ops.hip.adapter_outer(x, dz, groups.ids, groups.plan, e, r, True)
         if need_b:
-            db = ops.hip.adapter_outer(dy, z, groups.plan, e, r, False)
+            db = ops.hip.adapter_outer(dy, z, groups.ids, groups.plan, e, r, False)
         return (dy if need_base else None, dx, da, db) + (None,) * 4
 
 

@@ -66,15 +66,16 @@ torch::Tensor logprobs_bwd(torch::Tensor logits, torch::Tensor tokens,
 // adapter.hip — low-rank adapters of many requests
 torch::Tensor adapter_plan(torch::Tensor ids, int64_t E);
 torch::Tensor adapter_shrink(torch::Tensor x, torch::Tensor w,
-                             torch::Tensor plan,
+                             torch::Tensor ids, torch::Tensor plan,
                              c10::optional<torch::Tensor> scales,
                              double scale, bool kmajor);
 torch::Tensor adapter_expand(c10::optional<torch::Tensor> base,
                              torch::Tensor z, torch::Tensor w,
-                             torch::Tensor plan, int64_t act, bool rmajor);
+                             torch::Tensor ids, torch::Tensor plan,
+                             int64_t act, bool rmajor);
 torch::Tensor adapter_outer(torch::Tensor x, torch::Tensor z,
-                            torch::Tensor plan, int64_t E, int64_t R,
-                            bool kmajor);
+                            torch::Tensor ids, torch::Tensor plan, int64_t E,
+                            int64_t R, bool kmajor);
 torch::Tensor adapter_act_bwd(torch::Tensor y, torch::Tensor dy,
                               int64_t act);
 
@@ -232,11 +233,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "rows grouped by adapter: order, groups and tiles of 16 rows");
   m.def("adapter_shrink", &adapter_shrink,
         "z = scale * x w^T by adapter, fp32, in grouped order",
-        py::arg("x"), py::arg("w"), py::arg("plan"), py::arg("scales"),
-        py::arg("scale"), py::arg("kmajor"));
+        py::arg("x"), py::arg("w"), py::arg("ids"), py::arg("plan"),
+        py::arg("scales"), py::arg("scale"), py::arg("kmajor"));
   m.def("adapter_expand", &adapter_expand,
         "act(base + z w^T) by adapter", py::arg("base"), py::arg("z"),
-        py::arg("w"), py::arg("plan"), py::arg("act"), py::arg("rmajor"));
+        py::arg("w"), py::arg("ids"), py::arg("plan"), py::arg("act"),
+        py::arg("rmajor"));
   m.def("adapter_outer", &adapter_outer,
         "sums of z^T x over each adapter's rows");
   m.def("adapter_act_bwd", &adapter_act_bwd,

@@ -450,8 +450,9 @@ def _check_adapter(base, x, a, b, ids, scale, seed=50):
     return y, grads
 
 
-@pytest.mark.parametrize("m,e", [(0, 1), (1, 1), (5, 3), (16, 2), (17, 1),
-                                 (300, 4), (1000, 1024), (4097, 5)])
+@pytest.mark.parametrize("m,e", [(65, 1), (80, 3), (300, 4), (1000, 1024),
+                                 (4097, 5), (40000, 300), (8192, 8),
+                                 (8193, 640)])
 def test_adapter_plan(m, e):
     gen = torch.Generator().manual_seed(m)
     ids = torch.randint(-2, e + 2, (m,), generator=gen)
