@@ -44,12 +44,14 @@ __device__ __forceinline__ int group_of(long id, int E) {
 struct Plan {
   const long* ids;  // [M]
   int M, E;
-  int* perm;        // [M] the row at each place of the grouped order
-  int* seg;         // [E + 3] where a group's rows begin
-  int* tbase;       // [E + 3] where a group's tiles begin
-  int* tile_group;  // [tiles] -1 behind the last
-  int* tile_place;  // [tiles] first place
+  int4* tiles;   // up to 16 rows: group (-1 behind the last), first place, rows
+  int4* blocks;  // up to 64 rows, the same
+  int* perm;     // [M] the row at each place of the grouped order
+  int* seg;      // [E + 3] where a group's rows begin
+  int* tbase;    // [E + 3] where its tiles begin
 };
+
+#define BLOCK_TILES 4  // tiles of a block
 
 #define SMALL_ROWS 64
 
@@ -60,15 +62,11 @@ struct Tile {
   int g, rows, place, row;
 };
 
-// Tile t of a prepared plan, moved on by `sub` tiles of its group; the
-// caller makes sure that the group has them.
-__device__ __forceinline__ Tile plan_tile(const Plan& p, int t, int sub,
+// Tile `sub` of the rows that an entry of the plan names.
+__device__ __forceinline__ Tile plan_tile(const Plan& p, int4 of, int sub,
                                           int lane) {
-  Tile r = {p.tile_group[t], 0, 0, 0};
-  if (r.g < 0) return r;
-  const int first = p.tile_place[t] + sub * TILE;
-  r.rows = min(TILE, p.seg[r.g + 1] - first);
-  r.place = first + min(lane & 15, r.rows - 1);
+  Tile r = {of.x, min(TILE, of.z - sub * TILE), 0, 0};
+  r.place = of.y + sub * TILE + min(lane & 15, r.rows - 1);
   r.row = p.perm[r.place];
   return r;
 }
@@ -112,10 +110,11 @@ __device__ __forceinline__ unsigned long same_group(int g, int bits) {
 // 64 rows at once (8192 rows of 8 or 32 adapters, shuffled or in runs: one
 // batch a wave).
 __global__ void __launch_bounds__(PLAN_WAVES* WAVE)
-    adapter_plan_kernel(Plan p, int tiles, int waves) {
-  extern __shared__ int hist[];  // [waves][E + 2] and [E + 3]
+    adapter_plan_kernel(Plan p, int tiles, int blocks, int waves) {
+  extern __shared__ int hist[];  // [waves][E + 2] and three of [E + 3]
   const int M = p.M, E = p.E, G = E + 2;
   int* total = hist + waves * G;
+  int* tbase = total + G + 1;
   const int tid = threadIdx.x, wave = tid / WAVE, lane = tid & (WAVE - 1);
   const int threads = waves * WAVE;
   const int bits = 32 - __clz(G);
@@ -167,45 +166,57 @@ __global__ void __launch_bounds__(PLAN_WAVES* WAVE)
   }
   __syncthreads();
   // the first wave sums over the groups, 64 at a time
+  int* bbase = tbase + G + 1;
   if (wave == 0) {
-    int rows = 0, blocks = 0;
+    int rows = 0, nt = 0, nb = 0;
     for (int g0 = 0; g0 < G; g0 += WAVE) {
       const int g = g0 + lane;
       const int c = g < G ? total[g] : 0;
-      const int b = (c + TILE - 1) / TILE;
-      int cs = c, bs = b;
+      const int t = (c + TILE - 1) / TILE;
+      const int b = (t + BLOCK_TILES - 1) / BLOCK_TILES;
+      int cs = c, ts = t, bs = b;
 #pragma unroll
       for (int off = 1; off < WAVE; off <<= 1) {
         const int cu = __shfl_up(cs, off, WAVE);
+        const int tu = __shfl_up(ts, off, WAVE);
         const int bu = __shfl_up(bs, off, WAVE);
         if (lane >= off) {
           cs += cu;
+          ts += tu;
           bs += bu;
         }
       }
       if (g < G) {
         p.seg[g] = total[g] = rows + cs - c;
-        p.tbase[g] = blocks + bs - b;
+        p.tbase[g] = tbase[g] = nt + ts - t;
+        bbase[g] = nb + bs - b;
       }
       rows += __shfl(cs, WAVE - 1, WAVE);
-      blocks += __shfl(bs, WAVE - 1, WAVE);
+      nt += __shfl(ts, WAVE - 1, WAVE);
+      nb += __shfl(bs, WAVE - 1, WAVE);
     }
     if (lane == 0) {
       p.seg[G] = total[G] = rows;
-      p.tbase[G] = blocks;
+      p.tbase[G] = tbase[G] = nt;
+      bbase[G] = nb;
     }
-    for (int t = blocks + lane; t < tiles; t += WAVE) p.tile_group[t] = -1;
   }
   __syncthreads();
-  // a wave a group writes its tiles
+  // a wave a group writes its tiles and blocks
   for (int g = wave; g < G; g += waves) {
-    const int r0 = total[g], b0 = p.tbase[g];
-    const int b = (total[g + 1] - r0 + TILE - 1) / TILE;
-    for (int j = lane; j < b; j += WAVE) {
-      p.tile_group[b0 + j] = g;
-      p.tile_place[b0 + j] = r0 + j * TILE;
-    }
+    const int r0 = total[g], n = total[g + 1] - r0;
+    for (int j = lane; j * TILE < n; j += WAVE)
+      p.tiles[tbase[g] + j] =
+          make_int4(g, r0 + j * TILE, min(TILE, n - j * TILE), 0);
+    constexpr int ROWS = BLOCK_TILES * TILE;
+    for (int j = lane; j * ROWS < n; j += WAVE)
+      p.blocks[bbase[g] + j] =
+          make_int4(g, r0 + j * ROWS, min(ROWS, n - j * ROWS), 0);
   }
+  for (int t = tbase[G] + tid; t < tiles; t += threads)
+    p.tiles[t] = make_int4(-1, 0, 0, 0);
+  for (int t = bbase[G] + tid; t < blocks; t += threads)
+    p.blocks[t] = make_int4(-1, 0, 0, 0);
   // each wave places its stretch in order
   for (int i0 = lo; i0 < hi; i0 += PLAN_BATCH * WAVE) {
     if (hi - lo > PLAN_BATCH * WAVE) fetch(i0);  // else it holds them yet
@@ -246,6 +257,27 @@ __device__ __forceinline__ f32x4 mma(Vec<f16_t>::V a, Vec<f16_t>::V b,
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+// bf16 has the exponents of fp32, so three of them hold an fp32 number's 24
+// bits exactly: products of z with bf16 weights or rows go through the bf16
+// instruction three times at an eighth of the fp32 instruction's time each.
+// (fp16 has not the exponents: its products are taken in fp32.)
+struct Split {
+  Vec<bf16_t>::V high, mid, low;
+};
+
+__device__ __forceinline__ Split split(const float (&x)[8]) {
+  Split s;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    s.high[j] = (bf16_t)x[j];
+    // an infinity has no rest: inf - inf would make it NaN
+    const float a = fabsf(x[j]) <= 3.0e38f ? x[j] - (float)s.high[j] : 0.0f;
+    s.mid[j] = (bf16_t)a;
+    s.low[j] = (bf16_t)(a - (float)s.mid[j]);
+  }
+  return s;
+}
+
 // -- shrink -------------------------------------------------------------------
 
 // z[place][r] = s_e sum_k x[row][k] W_e(r, k).  W is [R, K] (KMAJOR) or
@@ -267,26 +299,29 @@ __global__ void __launch_bounds__(WAVES * WAVE)
   if (SMALL) {
     t[0] = small_tile(p, blockIdx.x, lane);
     if (t[0].g < 0 || t[0].g >= p.E) return;
+  } else if (SUB == 1) {
+    const int4 of = p.tiles[blockIdx.x];
+    if (of.x < 0 || of.x >= p.E) return;
+    t[0] = plan_tile(p, of, 0, lane);
   } else {
-    const int g = p.tile_group[blockIdx.x];
-    if (g < 0 || g >= p.E) return;
-    const int at = blockIdx.x - p.tbase[g];
-    if (at % SUB != 0) return;
+    constexpr int PARTS = BLOCK_TILES / SUB;
+    const int4 of = p.blocks[blockIdx.x / PARTS];
+    const int first = blockIdx.x % PARTS * SUB;
+    if (of.x < 0 || of.x >= p.E || first * TILE >= of.z) return;
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
-      // a tile that the group does not have repeats the first, unwritten
-      const bool has = (int)blockIdx.x + s < p.tbase[g + 1];
-      t[s] = plan_tile(p, blockIdx.x, has ? s : 0, lane);
+      // a tile that is not there repeats the first and is not written
+      const bool has = (first + s) * TILE < of.z;
+      t[s] = plan_tile(p, of, has ? first + s : first, lane);
       if (!has) t[s].rows = 0;
     }
   }
-  const int g = t[0].g;
   const int i = lane & 15, quarter = lane >> 4;
   // ranks behind R repeat the last; they are written as zero
   const T* xr[SUB];
 #pragma unroll
   for (int s = 0; s < SUB; ++s) xr[s] = x + (long)t[s].row * xstride;
-  const T* we = w + (long)g * R * K;
+  const T* we = w + (long)t[0].g * R * K;
   auto load_w = [&](int rb, int k) -> V {
     const int r = min(rb * 16 + i, R - 1);
     if (KMAJOR) return Vec<T>::load(we + (long)r * K + k);
@@ -297,7 +332,12 @@ __global__ void __launch_bounds__(WAVES * WAVE)
   };
   f32x4 acc[SUB][RB] = {};
   const int whole = K / (STEP * U);
-  for (int c = wave; c < whole; c += WAVES) {
+  // Every block starts elsewhere in its rows: rows lie a power of two apart
+  // as a rule, and blocks that walk them in step meet in a few channels of
+  // the memory.
+  const int turn = whole > 0 ? (int)blockIdx.x * WAVES % whole : 0;
+  for (int c0 = wave; c0 < whole; c0 += WAVES) {
+    const int c = c0 + turn < whole ? c0 + turn : c0 + turn - whole;
     V xv[U][SUB], wv[U][RB];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -351,7 +391,7 @@ __global__ void __launch_bounds__(WAVES * WAVE)
     for (int rb = 0; rb < RB; ++rb)
       part[wave][s * RB + rb][lane] = acc[s][rb];
   __syncthreads();
-  const float f = scales ? scales[g] : scale;
+  const float f = scales ? scales[t[0].g] : scale;
   // whole waves: a wave's 64 lanes finish the 16 x 16 of one (s, rb)
   for (int b = wave; b < SUB * RB; b += WAVES) {
     f32x4 sum = part[0][b][lane];
@@ -381,137 +421,274 @@ __device__ __forceinline__ float act_keep_nan(float x, int act) {
 // -- expand -------------------------------------------------------------------
 
 // out[row][n] = act(base[row][n] + sum_r z[place][r] W_e(n, r)), W [N, R]
-// (RMAJOR) or [R, N].  One block takes 16 V columns of up to WAVES tiles of
-// an adapter, a wave a tile, and lays its part of W into LDS once as [n][r].
-// The product is taken as D[n][m], in fp32; instruction j's row 4 h + q is
-// column 4 V a + V h + e of the block's, where j = a V / 4 + e / 4 and
-// q = e % 4, so that a lane ends up with 16 bytes of adjacent outputs and
-// its row's four lanes with 64.  base enters as the sum's first term.
+// (RMAJOR) or [R, N].  One block takes up to WAVES tiles of an adapter, a
+// wave a tile, through chunks of 16 V columns; a chunk's part of W is laid
+// into LDS as it lies in memory, and the loads of the next chunk are under
+// way during this one's products.  The product is taken as D[n][m], in
+// fp32; instruction j's row 4 h + q is the chunk's column
+// 4 V a + V h + e, where j = a V / 4 + e / 4 and q = e % 4, so that a lane
+// ends up with 16 bytes of adjacent outputs and its row's four lanes with
+// 64.  base enters as the sum's first term.
 template <typename T, int RB, bool RMAJOR, int WAVES>
 __global__ void __launch_bounds__(WAVES * WAVE)
     adapter_expand_kernel(const T* __restrict__ base, long bstride,
                           const float* __restrict__ z,
                           const T* __restrict__ w, Plan p,
-                          T* __restrict__ out, int N, int R, int act) {
+                          T* __restrict__ out, int N, int R, int act,
+                          int across) {
   constexpr int V = Vec<T>::N;
   constexpr int COLS = 16 * V;
-  constexpr int PITCH = 16 * RB + 16 / sizeof(T);  // of a column in LDS
+  constexpr int THREADS = WAVES * WAVE;
   constexpr bool SMALL = WAVES == 1;
   typedef typename Vec<T>::V VT;
   typedef T T4 __attribute__((ext_vector_type(4)));
-  __shared__ __attribute__((aligned(16))) T wl[COLS * PITCH];
+  struct __attribute__((packed, aligned(sizeof(T)))) U4 {
+    T4 v;
+  };
+  // bf16: 16 bytes of ranks an operand, so [R, N] is turned round on its
+  // way into LDS
+  constexpr bool BF16 = std::is_same<T, bf16_t>::value;
+  constexpr bool TURN = BF16 && !RMAJOR;
+  // LDS: a column's ranks side by side, or a rank's columns; the pitch
+  // spreads a wave's quarters over the banks
+  constexpr int PITCH = RMAJOR || TURN ? 16 * RB + 16 / sizeof(T)
+                                       : COLS + 16 / sizeof(T);
+  constexpr int PART = RMAJOR || TURN ? COLS * PITCH : 16 * RB * PITCH;
+  constexpr int BUFFERS = 2 * PART * sizeof(T) <= 49152 ? 2 : 1;
+  // vectors of W that a thread takes: 4 ranks; V columns; V columns of four
+  // ranks
+  constexpr int ALL = RMAJOR ? COLS * 4 * RB : TURN ? 64 * RB : 256 * RB;
+  constexpr int TAKE = ALL < THREADS ? 1 : ALL / THREADS;
+  constexpr int WIDE = TURN ? 4 : 1;
+  __shared__ __attribute__((aligned(16))) T wl[BUFFERS][PART];
   const int tid = threadIdx.x;
   const int lane = tid & (WAVE - 1), wave = tid / WAVE;
   const int i = lane & 15, quarter = lane >> 4;
-  const int n0 = blockIdx.y * COLS;
+  // the columns' blocks are neighbours: blocks of different rows that run
+  // side by side would write the same channels of the memory
+  const int block = blockIdx.x / across, first = blockIdx.x % across;
   Tile t;
-  int g;
   bool has = true;
   if (SMALL) {
-    t = small_tile(p, blockIdx.x, lane);
-    g = t.g;
-    if (g < 0) return;
+    t = small_tile(p, block, lane);
+    if (t.g < 0) return;
   } else {
-    g = p.tile_group[blockIdx.x];
-    if (g < 0 || (blockIdx.x - p.tbase[g]) % WAVES != 0) return;
-    has = (int)blockIdx.x + wave < p.tbase[g + 1];
-    t = plan_tile(p, blockIdx.x, has ? wave : 0, lane);
+    const int4 of = p.blocks[block];
+    if (of.x < 0) return;
+    has = wave * TILE < of.z;
+    t = plan_tile(p, of, has ? wave : 0, lane);
   }
+  const int g = t.g;
+  const bool adapted = g < p.E;
   const bool mine = has && i < t.rows;
-  const int out0 = n0 + V * quarter;
-  VT bv[4];
-  if (base != nullptr && mine) {
-    const T* br = base + (long)t.row * bstride + out0;
+  const T* br = base + (long)t.row * bstride;
+  T* orow = out + (long)t.row * N;
+  const T* we = w + (long)(adapted ? g : 0) * N * R;
+
+  VT bv[4], bn[4];
+  // Only the last chunk has vectors to cut: the others load without
+  // branches.
+  auto load_base = [&](int n0) {
+    if (base == nullptr) return;
+    const int c0 = n0 + V * quarter;
+    if (n0 + COLS <= N) {
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      if (out0 + 4 * V * a + V <= N) {
-        bv[a] = Vec<T>::load(br + 4 * V * a);
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          bv[a][e] = out0 + 4 * V * a + e < N ? br[4 * V * a + e] : (T)0.0f;
-      }
+      for (int a = 0; a < 4; ++a) bn[a] = Vec<T>::load(br + c0 + 4 * V * a);
+      return;
     }
-  }
-  f32x4 zv[RB];
-  if (g < p.E) {
 #pragma unroll
-    for (int c = 0; c < RB; ++c)
-      zv[c] = *reinterpret_cast<const f32x4*>(
-          z + (long)t.place * (RB * 16) + 16 * c + 4 * quarter);
-    const T* we = w + (long)g * N * R;
-    if (RMAJOR) {
-      // ranks in fours: a vector where the rank has all four
-      for (int at = tid; at < COLS * 4 * RB; at += WAVES * WAVE) {
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int c = c0 + 4 * V * a + e;
+        bn[a][e] = c < N ? br[c] : (T)0.0f;
+      }
+  };
+  // [R, N]: neighbouring lanes take neighbouring columns; turned round,
+  // neighbouring ranks, which lie side by side in LDS (the other way round
+  // eight lanes meet in a bank)
+  auto rank_of = [](int at) { return TURN ? at % (4 * RB) * 4 : at / 16; };
+  auto column_of = [](int at) {
+    return (TURN ? at / (4 * RB) : at % 16) * V;
+  };
+  T4 w4[RMAJOR ? TAKE : 1];
+  VT wv[RMAJOR ? 1 : TAKE][WIDE];
+  auto load_w = [&](int n0) {
+    if (!adapted) return;
+    if (n0 + COLS <= N && R == 16 * RB) {
+#pragma unroll
+      for (int u = 0; u < TAKE; ++u) {
+        const int at = tid + u * THREADS;
+        if (RMAJOR) {  // the chunk is one piece of memory
+          w4[u] = reinterpret_cast<const U4*>(we + (long)n0 * R + at * 4)->v;
+        } else if (at < ALL) {
+#pragma unroll
+          for (int q = 0; q < WIDE; ++q)
+            wv[u][q] = Vec<T>::load(we + (long)(rank_of(at) + q) * N + n0 +
+                                    column_of(at));
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int u = 0; u < TAKE; ++u) {
+      const int at = tid + u * THREADS;
+      if (RMAJOR) {
         const int c = at / (4 * RB), r = at % (4 * RB) * 4;
         const T* wr = we + (long)min(n0 + c, N - 1) * R + r;
-        T4 v;
-        if (r + 4 <= R) {
-          struct __attribute__((packed, aligned(sizeof(T)))) U4 {
-            T4 v;
-          };
-          v = reinterpret_cast<const U4*>(wr)->v;
-        } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = r + e < R ? wr[e] : (T)0.0f;
+        for (int e = 0; e < 4; ++e) w4[u][e] = r + e < R ? wr[e] : (T)0.0f;
+      } else {
+#pragma unroll
+        for (int q = 0; q < WIDE; ++q) {
+          const int r = rank_of(at) + q, c = n0 + column_of(at);
+          const T* wr = we + (long)r * N + c;
+          if (r < R && c + V <= N) {
+            wv[u][q] = Vec<T>::load(wr);
+          } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+              wv[u][q][e] = r < R && c + e < N ? wr[e] : (T)0.0f;
+          }
         }
-        *reinterpret_cast<T4*>(&wl[c * PITCH + r]) = v;
       }
-    } else {
-      for (int at = tid; at < 16 * RB * 16; at += WAVES * WAVE) {
-        const int r = at / 16, c = at % 16 * V;
-        const T* wr = we + (long)min(r, R - 1) * N + n0 + c;
-        VT v;
-        if (n0 + c + V <= N) {
-          v = Vec<T>::load(wr);
-        } else {
+    }
+  };
+
+  const int step = across * COLS;
+  int n0 = first * COLS;
+  load_base(n0);
+  load_w(n0);
+  // z: fp32 four at a time; bf16 in parts, eight at a time.  A rank of 16
+  // fills only half of the 32 that a bf16 instruction sums over: there the
+  // high parts take one half and the middle parts the other.
+  constexpr int ZB = BF16 ? 1 : RB, ZP = BF16 ? (RB + 1) / 2 : 1;
+  f32x4 zv[ZB];
+  Vec<bf16_t>::V zh[ZP], zm[ZP], zl[ZP];
+  if (adapted && BF16) {
 #pragma unroll
-          for (int e = 0; e < V; ++e)
-            v[e] = n0 + c + e < N ? wr[e] : (T)0.0f;
+    for (int b = 0; b < ZP; ++b) {
+      const int r = 32 * b + 8 * (RB == 1 ? quarter & 1 : quarter);
+      const float* from = z + (long)t.place * (RB * 16) + r;
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(from);
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(from + 4);
+      const float f[8] = {lo[0], lo[1], lo[2], lo[3],
+                          hi[0], hi[1], hi[2], hi[3]};
+      const Split s = split(f);
+      zh[b] = s.high;
+      zm[b] = s.mid;
+      zl[b] = s.low;
+      if (RB == 1) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          zh[b][e] = quarter < 2 ? s.high[e] : s.mid[e];
+          zl[b][e] = quarter < 2 ? s.low[e] : (bf16_t)0.0f;
+        }
+      }
+    }
+  } else if (adapted) {
+#pragma unroll
+    for (int c = 0; c < ZB; ++c)
+      zv[c] = *reinterpret_cast<const f32x4*>(
+          z + (long)t.place * (RB * 16) + 16 * c + 4 * quarter);
+  }
+  for (int turn = 0; n0 < N; n0 += step, ++turn) {
+    T* const part = wl[turn % BUFFERS];
+    if (BUFFERS == 1) __syncthreads();  // the last chunk's part was read
+    if (adapted) {
+#pragma unroll
+      for (int u = 0; u < TAKE; ++u) {
+        const int at = tid + u * THREADS;
+        if (RMAJOR) {
+          *reinterpret_cast<T4*>(
+              &part[at / (4 * RB) * PITCH + at % (4 * RB) * 4]) = w4[u];
+        } else if (TURN) {
+          if (at < ALL) {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+              *reinterpret_cast<T4*>(
+                  &part[(column_of(at) + e) * PITCH + rank_of(at)]) =
+                  T4{wv[u][0][e], wv[u][1 % WIDE][e], wv[u][2 % WIDE][e],
+                     wv[u][3 % WIDE][e]};
+          }
+        } else {
+          *reinterpret_cast<VT*>(
+              &part[rank_of(at) * PITCH + column_of(at)]) = wv[u][0];
+        }
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < 4; ++a) bv[a] = bn[a];
+    __syncthreads();
+    if (n0 + step < N) {
+      load_base(n0 + step);
+      load_w(n0 + step);
+    }
+    f32x4 acc[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      constexpr int H = V / 4;  // instructions to a vector of the output
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        acc[j][q] =
+            base != nullptr ? (float)bv[j / H][4 * (j % H) + q] : 0.0f;
+      if (adapted) {
+        const int c = 4 * V * (j / H) + V * (i >> 2) + 4 * (j % H) + (i & 3);
+        if constexpr (BF16) {
+#pragma unroll
+          for (int b = 0; b < ZP; ++b) {
+            const VT v = *reinterpret_cast<const VT*>(
+                &part[c * PITCH + 32 * b +
+                      8 * (RB == 1 ? quarter & 1 : quarter)]);
+            acc[j] = mma(v, zl[b], acc[j]);
+            if (RB > 1) acc[j] = mma(v, zm[b], acc[j]);
+            acc[j] = mma(v, zh[b], acc[j]);
+          }
+          continue;
         }
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          wl[(c + e) * PITCH + r] = r < R ? v[e] : (T)0.0f;
+        for (int b = 0; b < ZB; ++b) {
+          const int r = 16 * b + 4 * quarter;
+          T4 v;
+          if (RMAJOR) {
+            v = *reinterpret_cast<const T4*>(&part[c * PITCH + r]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = part[(r + e) * PITCH + c];
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                (float)v[e], zv[b][e], acc[j], 0, 0, 0);
+        }
       }
     }
-  }
-  __syncthreads();
-  f32x4 acc[V];
+    const int c0 = n0 + V * quarter;
+    if (g > p.E) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    constexpr int H = V / 4;  // instructions to a vector of the output
+      for (int j = 0; j < V; ++j) acc[j] = f32x4{NAN, NAN, NAN, NAN};
+    } else if (act != ACT_NONE) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      acc[j][q] = base != nullptr ? (float)bv[j / H][4 * (j % H) + q] : 0.0f;
-    if (g < p.E) {
-      const int c = 4 * V * (j / H) + V * (i >> 2) + 4 * (j % H) + (i & 3);
+      for (int j = 0; j < V; ++j)
 #pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        const T4 v = *reinterpret_cast<const T4*>(
-            &wl[c * PITCH + 16 * b + 4 * quarter]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-              (float)v[e], zv[b][e], acc[j], 0, 0, 0);
-      }
+        for (int q = 0; q < 4; ++q) acc[j][q] = act_keep_nan(acc[j][q], act);
     }
-  }
-  if (!mine) return;
-  T* o = out + (long)t.row * N + out0;
+    VT v[4];
 #pragma unroll
-  for (int a = 0; a < 4; ++a) {
-    VT v;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float y = g > p.E ? NAN : acc[a * (V / 4) + e / 4][e % 4];
-      v[e] = (T)act_keep_nan(y, act);
-    }
-    if (out0 + 4 * V * a + V <= N) {
-      Vec<T>::store(o + 4 * V * a, v);
-    } else {
+    for (int a = 0; a < 4; ++a)
 #pragma unroll
       for (int e = 0; e < V; ++e)
-        if (out0 + 4 * V * a + e < N) o[4 * V * a + e] = v[e];
+        v[a][e] = (T)acc[a * (V / 4) + e / 4][e % 4];
+    if (!mine) continue;
+    if (n0 + COLS <= N) {
+#pragma unroll
+      for (int a = 0; a < 4; ++a) Vec<T>::store(orow + c0 + 4 * V * a, v[a]);
+    } else {
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (c0 + 4 * V * a + e < N) orow[c0 + 4 * V * a + e] = v[a][e];
     }
   }
 }
@@ -527,10 +704,11 @@ __device__ __forceinline__ int first_slot(const Plan& p, int e,
   return p.tbase[e] / stretch + e;
 }
 
-// sum over the rows of a stretch of one adapter: z[place][r] x[row][k], with
-// fp32 products.  A lane loads 16 bytes of a row; instruction j takes
-// element j of all lanes, so its 16 columns are k0 + V (l % 16) + j and its
-// four k are four rows.  KMAJOR: the result is [R, K] (dA), else [K, R]
+// sum over the rows of a stretch of one adapter: z[place][r] x[row][k].  A
+// lane loads 16 bytes of a row; instruction j takes element j of all lanes,
+// so its 16 columns are k0 + V (l % 16) + j.  Its sum runs over four rows in
+// fp32; in bf16 over 32, of which a lane has every fourth: eight loads, whose
+// elements j are one operand, beside z in three parts.  KMAJOR: the result is [R, K] (dA), else [K, R]
 // (dB).  SMALL_OUTER, DIRECT_OUTER: one block an adapter, rounded into out;
 // SPLIT_OUTER: one block a stretch, into fp32 sums that reduce joins.
 template <typename T, int RB, bool KMAJOR, OuterWork WORK>
@@ -540,7 +718,8 @@ __global__ void __launch_bounds__(256)
                          T* __restrict__ out, float* __restrict__ partial,
                          int K, int R, int stretch) {
   constexpr int V = Vec<T>::N;
-  constexpr int U = 4;
+  constexpr bool BF16 = std::is_same<T, bf16_t>::value;
+  constexpr int U = BF16 ? 8 : 4;
   __shared__ f32x4 part[2][RB * V][WAVE];
   __shared__ int list[SMALL_ROWS];
   __shared__ int found;
@@ -548,23 +727,23 @@ __global__ void __launch_bounds__(256)
   const int i = lane & 15, quarter = lane >> 4;
   int begin = 0, end = 0;
   if (WORK == SMALL_OUTER) {
-    const bool here = lane < p.M && p.ids[lane] == (long)blockIdx.x;
+    const bool here = lane < p.M && p.ids[lane] == (long)blockIdx.y;
     const unsigned long all = __ballot(here);
     if (here && wave == 0) list[__popcll(all & ((1ul << lane) - 1))] = lane;
     end = __popcll(all);
     __syncthreads();
   } else if (WORK == DIRECT_OUTER) {
-    begin = p.seg[blockIdx.x];
-    end = p.seg[blockIdx.x + 1];
+    begin = p.seg[blockIdx.y];
+    end = p.seg[blockIdx.y + 1];
   } else {
     if (threadIdx.x == 0) found = -1;
     __syncthreads();
     for (int e = threadIdx.x; e < p.E; e += 256) {
-      const int c = (int)blockIdx.x - first_slot(p, e, stretch);
+      const int c = (int)blockIdx.y - first_slot(p, e, stretch);
       const int n = p.tbase[e + 1] - p.tbase[e];
       if (c >= 0 && c * stretch < n) {
         found = e;
-        list[0] = p.tile_place[p.tbase[e] + c * stretch];
+        list[0] = p.seg[e] + c * stretch * TILE;
       }
     }
     __syncthreads();
@@ -573,69 +752,155 @@ __global__ void __launch_bounds__(256)
     end = min(p.seg[found + 1], begin + stretch * TILE);
   }
   const int r0 = blockIdx.z * (RB * 16);
-  const int k0 = blockIdx.y * (16 * V);
+  const int k0 = blockIdx.x * (16 * V);
   const int k = k0 + i * V;
   f32x4 acc[RB][V] = {};
-  // Four rows an instruction, U times four a step.  The next step's rows
-  // are loaded before this one's products, and their numbers a step before
-  // that.
-  int place[U], row[U];
-  auto number = [&](int m0) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
+  // The bf16 loop: 32 rows a step.  Nothing but the rows' numbers is loaded
+  // a step ahead: the registers go into a third wave a SIMD instead.
+  auto steps32 = [&](auto whole) {
+    if constexpr (BF16) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    constexpr int STEP = 4 * 32;  // of the four waves
+    int row[U];
+    auto place = [&](int m0, int u) {
       const int at = min(m0 + 4 * u + quarter, end - 1);
-      place[u] = WORK == SMALL_OUTER ? list[at] : at;
-      row[u] = WORK == SMALL_OUTER ? place[u] : p.perm[at];
-    }
-  };
-  typename Vec<T>::V xv[U], xn[U];
-  float zv[U][RB], zn[U][RB];
-  auto load = [&]() {
+      return WORK == SMALL_OUTER ? list[at] : at;
+    };
+    auto number = [&](int m0) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const T* xr = x + (long)row[u] * xstride;
-      if (k + V <= K) {
-        xn[u] = Vec<T>::load(xr + k);
-      } else {
+      for (int u = 0; u < U; ++u)
+        row[u] = WORK == SMALL_OUTER ? place(m0, u) : p.perm[place(m0, u)];
+    };
+    int m0 = begin + wave * 32;
+    if (m0 < end) number(m0);
+    for (; m0 < end; m0 += STEP) {
+      typename Vec<T>::V xv[U];
+      float zv[RB][U];
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          xn[u][j] = k + j < K ? xr[k + j] : (T)0.0f;
+      for (int u = 0; u < U; ++u) {
+        const T* xr = x + (long)row[u] * xstride;
+        if (WHOLE) {
+          xv[u] = Vec<T>::load(xr + k);
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            xv[u][j] = k + j < K ? xr[k + j] : (T)0.0f;
+        }
       }
 #pragma unroll
-      for (int c = 0; c < RB; ++c)
-        zn[u][c] = z[(long)place[u] * zstride + r0 + 16 * c + i];
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int c = 0; c < RB; ++c)
+          zv[c][u] = z[(long)place(m0, u) * zstride + r0 + 16 * c + i];
+      number(m0 + STEP);
+      if (m0 + 32 > end) {
+        // rows behind the last: both factors, since 0 x NaN is not 0
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const bool in = m0 + 4 * u + quarter < end;
+#pragma unroll
+          for (int j = 0; j < V; ++j) xv[u][j] = in ? xv[u][j] : (T)0.0f;
+#pragma unroll
+          for (int c = 0; c < RB; ++c) zv[c][u] = in ? zv[c][u] : 0.0f;
+        }
+      }
+      Split zs[RB];
+#pragma unroll
+      for (int c = 0; c < RB; ++c) zs[c] = split(zv[c]);
+#pragma unroll
+      for (int j = 0; j < V; j += 2) {
+        typename Vec<T>::V col[2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          col[0][u] = xv[u][j];
+          col[1][u] = xv[u][j + 1];
+        }
+#pragma unroll
+        for (int part = 0; part < 3; ++part)
+#pragma unroll
+          for (int c = 0; c < RB; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              acc[c][j + h] = mma(part == 0   ? zs[c].low
+                                  : part == 1 ? zs[c].mid
+                                              : zs[c].high,
+                                  col[h], acc[c][j + h]);
+      }
+    }
+  }
+  };
+  // Four rows an instruction, U times four a step.  The next step's rows
+  // are loaded before this one's products, and their numbers a step before
+  // that.  Only the last columns' block has vectors to cut: the others take
+  // a loop without branches.
+  auto steps = [&](auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    int place[U], row[U];
+    auto number = [&](int m0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int at = min(m0 + 4 * u + quarter, end - 1);
+        place[u] = WORK == SMALL_OUTER ? list[at] : at;
+        row[u] = WORK == SMALL_OUTER ? place[u] : p.perm[at];
+      }
+    };
+    typename Vec<T>::V xv[U], xn[U];
+    float zv[U][RB], zn[U][RB];
+    auto load = [&]() {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const T* xr = x + (long)row[u] * xstride;
+        if (WHOLE) {
+          xn[u] = Vec<T>::load(xr + k);
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            xn[u][j] = k + j < K ? xr[k + j] : (T)0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < RB; ++c)
+          zn[u][c] = z[(long)place[u] * zstride + r0 + 16 * c + i];
+      }
+    };
+    constexpr int STEP = 16 * U;
+    int m0 = begin + wave * 4 * U;
+    if (m0 < end) {
+      number(m0);
+      load();
+      number(m0 + STEP);
+    }
+    for (; m0 < end; m0 += STEP) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool in = m0 + 4 * u + quarter < end;
+        // rows behind the last: both factors, since 0 x NaN is not 0
+#pragma unroll
+        for (int j = 0; j < V; ++j) xv[u][j] = in ? xn[u][j] : (T)0.0f;
+#pragma unroll
+        for (int c = 0; c < RB; ++c) zv[u][c] = in ? zn[u][c] : 0.0f;
+      }
+      load();  // behind the last step: rows that are there, not used
+      number(m0 + 2 * STEP);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int c = 0; c < RB; ++c)
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                zv[u][c], (float)xv[u][j], acc[c][j], 0, 0, 0);
     }
   };
-  constexpr int STEP = 16 * U;
-  int m0 = begin + wave * 4 * U;
-  if (m0 < end) {
-    number(m0);
-    load();
-    number(m0 + STEP);
-  }
-  for (; m0 < end; m0 += STEP) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = m0 + 4 * u + quarter < end;
-      // rows behind the last: both factors, since 0 x NaN is not 0
-#pragma unroll
-      for (int j = 0; j < V; ++j) xv[u][j] = in ? xn[u][j] : (T)0.0f;
-#pragma unroll
-      for (int c = 0; c < RB; ++c) zv[u][c] = in ? zn[u][c] : 0.0f;
-    }
-    if (m0 + STEP < end) {
-      load();
-      number(m0 + 2 * STEP);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int c = 0; c < RB; ++c)
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-              zv[u][c], (float)xv[u][j], acc[c][j], 0, 0, 0);
-  }
+  auto run = [&](auto whole) {
+    if constexpr (BF16)
+      steps32(whole);
+    else
+      steps(whole);
+  };
+  if (k0 + 16 * V <= K)
+    run(std::true_type());
+  else
+    run(std::false_type());
   // the four waves' sums meet in the first
 #pragma unroll
   for (int half = 2; half > 0; half >>= 1) {
@@ -656,24 +921,39 @@ __global__ void __launch_bounds__(256)
     }
   }
   if (wave != 0) return;
-  const long o0 = (long)blockIdx.x * R * K;
+  const long o0 = (long)blockIdx.y * R * K;
+  // KMAJOR: a lane has V adjacent columns of four ranks; else four adjacent
+  // ranks of V columns
 #pragma unroll
-  for (int c = 0; c < RB; ++c)
+  for (int c = 0; c < RB; ++c) {
+    const int r = r0 + 16 * c + 4 * quarter;
+    if (k + V <= K && r + 4 <= R && WORK == SPLIT_OUTER) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int r = r0 + 16 * c + 4 * quarter + q;
-      if (r >= R) continue;
+      for (int q = 0; KMAJOR && q < 4; ++q)
+#pragma unroll
+        for (int h = 0; h < V / 4; ++h)
+          Vec<float>::store(partial + o0 + (long)(r + q) * K + k + 4 * h,
+                            f32x4{acc[c][4 * h][q], acc[c][4 * h + 1][q],
+                                  acc[c][4 * h + 2][q],
+                                  acc[c][4 * h + 3][q]});
+#pragma unroll
+      for (int j = 0; !KMAJOR && j < V; ++j)
+        Vec<float>::store(partial + o0 + (long)(k + j) * R + r, acc[c][j]);
+      continue;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if (k + j >= K) continue;
-        const long o = o0 + (KMAJOR ? (long)r * K + k + j
-                                    : (long)(k + j) * R + r);
+        if (k + j >= K || r + q >= R) continue;
+        const long o = o0 + (KMAJOR ? (long)(r + q) * K + k + j
+                                    : (long)(k + j) * R + r + q);
         if (WORK == SPLIT_OUTER)
           partial[o] = acc[c][j][q];
         else
           out[o] = (T)acc[c][j][q];
       }
-    }
+  }
 }
 
 // out_e = the sum of adapter e's partial sums, in their order; zero for an
@@ -710,16 +990,21 @@ static long max_tiles(long M, long E) {
   return M / TILE + std::min(E + 2, M);
 }
 
-static long plan_size(long M, long E) {
-  return M <= SMALL_ROWS ? 0 : M + 2 * (E + 3) + 2 * max_tiles(M, E);
+static long max_blocks(long M, long E) {
+  return M / (BLOCK_TILES * TILE) + std::min(E + 2, M);
 }
 
-// perm, seg, tbase, tile_group, tile_place in one int32 tensor.
+static long plan_size(long M, long E) {
+  if (M <= SMALL_ROWS) return 0;
+  return 4 * (max_tiles(M, E) + max_blocks(M, E)) + M + 2 * (E + 3);
+}
+
+// tiles, blocks, perm, seg and tbase in one int32 tensor.
 static Plan plan_of(const torch::Tensor& ids, const torch::Tensor& plan,
                     long E) {
   TORCH_CHECK(ids.is_cuda() && ids.is_contiguous() && ids.dim() == 1 &&
                   ids.scalar_type() == torch::kInt64 &&
-                  ids.size(0) < (1l << 30),
+                  ids.size(0) < (1l << 28),
               "ids must be contiguous int64 [rows] on GPU");
   TORCH_CHECK(E >= 1 && E <= ADAPTERS_MAX, "1 .. 1024 adapters");
   const long M = ids.size(0);
@@ -730,11 +1015,11 @@ static Plan plan_of(const torch::Tensor& ids, const torch::Tensor& plan,
   Plan r = {ids.data_ptr<int64_t>(), (int)M, (int)E, nullptr, nullptr,
             nullptr, nullptr, nullptr};
   if (M > SMALL_ROWS) {
-    r.perm = plan.data_ptr<int>();
+    r.tiles = reinterpret_cast<int4*>(plan.data_ptr<int>());
+    r.blocks = r.tiles + max_tiles(M, E);
+    r.perm = reinterpret_cast<int*>(r.blocks + max_blocks(M, E));
     r.seg = r.perm + M;
     r.tbase = r.seg + E + 3;
-    r.tile_group = r.tbase + E + 3;
-    r.tile_place = r.tile_group + max_tiles(M, E);
   }
   return r;
 }
@@ -749,11 +1034,12 @@ torch::Tensor adapter_plan(torch::Tensor ids, int64_t E) {
   const Plan p = plan_of(ids, plan, E);
   if (M <= SMALL_ROWS) return plan;
   // 16 waves while their counts fit 48 KB of LDS, else 8
-  const int waves = PLAN_WAVES * (E + 2) + E + 3 <= 12288 ? PLAN_WAVES : 8;
-  const int lds = (int)((waves * (E + 2) + E + 3) * sizeof(int));
+  const long each = 3 * (E + 3);
+  const int waves = PLAN_WAVES * (E + 2) + each <= 12288 ? PLAN_WAVES : 8;
+  const int lds = (int)((waves * (E + 2) + each) * sizeof(int));
   hipLaunchKernelGGL(adapter_plan_kernel, dim3(1), dim3(waves * WAVE), lds,
                      at::cuda::getCurrentCUDAStream(), p,
-                     (int)max_tiles(M, E), waves);
+                     (int)max_tiles(M, E), (int)max_blocks(M, E), waves);
   LAUNCH_OK();
   return plan;
 }
@@ -830,16 +1116,18 @@ torch::Tensor adapter_shrink(torch::Tensor x, torch::Tensor w,
   if (M == 0) return z;
   auto stream = at::cuda::getCurrentCUDAStream();
   const bool small = M <= SMALL_ROWS;
-  const long tiles = small ? M : max_tiles(M, E);
   for_dtype(x.scalar_type(), "x", [&](auto t) {
     using T = decltype(t);
     for_rank(R, [&](auto rb) {
       constexpr int RB = decltype(rb)::value;
-      // loads of 16 bytes that a lane has in flight: U (SUB + RB)
+      // Loads of 16 bytes that a lane has in flight: U (1 + RB).  Two tiles
+      // a block halve the reads of W: at 8192 rows of 4096 bf16 and a rank
+      // of 32 that is 18.8 us for 25.5, at 16 25.8 for 17.9 (half as many
+      // blocks are left, and what a CU has under way is what bounds it).
       constexpr int U = RB == 1 ? 8 : RB == 2 ? 4 : 2;
       constexpr int MANY = RB <= 4 ? 16 : 8;  // waves whose sums fit the LDS
-      auto go = [&](auto kernel, int waves) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)tiles),
+      auto go = [&](auto kernel, int waves, long blocks) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks),
                            dim3(waves * WAVE), 0, stream, ptr<T>(x),
                            (long)x.stride(0), ptr<T>(w), p, sp, (float)scale,
                            z.data_ptr<float>(), (int)K, (int)R);
@@ -847,9 +1135,14 @@ torch::Tensor adapter_shrink(torch::Tensor x, torch::Tensor w,
       auto pick = [&](auto major) {
         constexpr bool KM = decltype(major)::value;
         if (small)
-          go(adapter_shrink_kernel<T, RB, KM, true, MANY, 1, U>, MANY);
+          go(adapter_shrink_kernel<T, RB, KM, true, MANY, 1, U>, MANY, M);
+        else if (M >= 4096 && (RB == 2 || RB == 4))
+          go(adapter_shrink_kernel<T, RB, KM, false, 8, RB <= 4 ? 2 : 1,
+                                   RB <= 4 ? 4 / RB : 1>,
+             8, BLOCK_TILES / 2 * max_blocks(M, E));
         else
-          go(adapter_shrink_kernel<T, RB, KM, false, 8, 1, U>, 8);
+          go(adapter_shrink_kernel<T, RB, KM, false, 8, 1, U>, 8,
+             max_tiles(M, E));
       };
       if (kmajor)
         pick(std::true_type());
@@ -881,20 +1174,25 @@ torch::Tensor adapter_expand(c10::optional<torch::Tensor> base,
   if (M == 0) return out;
   auto stream = at::cuda::getCurrentCUDAStream();
   const bool small = M <= SMALL_ROWS;
-  const long tiles = small ? M : max_tiles(M, E);
+  const long blocks = small ? M : max_blocks(M, E);
   for_dtype(w.scalar_type(), "adapters", [&](auto t) {
     using T = decltype(t);
     const long cols = 16 * Vec<T>::N;
     for_rank(R, [&](auto rb) {
       constexpr int RB = decltype(rb)::value;
       auto go = [&](auto kernel, int waves) {
+        // as many blocks across as leave 2048 in all: what is left of the
+        // columns a block takes in turns
+        const long chunks = (N + cols - 1) / cols;
+        long turns = std::max<long>(1, chunks * blocks / 2048);
+        const long across = (chunks + turns - 1) / turns;
+        TORCH_CHECK(blocks * across < (1l << 31), "too many rows");
         hipLaunchKernelGGL(
-            kernel,
-            dim3((unsigned)tiles, (unsigned)((N + cols - 1) / cols)),
+            kernel, dim3((unsigned)(blocks * across)),
             dim3(waves * WAVE), 0, stream,
             base.has_value() ? ptr<T>(*base) : nullptr,
             base.has_value() ? (long)base->stride(0) : 0l, zp, ptr<T>(w), p,
-            ptr<T>(out), (int)N, (int)R, (int)act);
+            ptr<T>(out), (int)N, (int)R, (int)act, (int)across);
       };
       if (rmajor && small)
         go(adapter_expand_kernel<T, RB, true, 1>, 1);
@@ -928,12 +1226,15 @@ torch::Tensor adapter_outer(torch::Tensor x, torch::Tensor z,
   auto stream = at::cuda::getCurrentCUDAStream();
   const long tiles = max_tiles(M, E);
   // Up to 1024 rows one block adds all of an adapter's; above, stretches
-  // that give about 1024 blocks, so that one busy adapter is not one block.
+  // that give about 512 blocks, so that one busy adapter is not one block
+  // (8192 rows of 4096 fp16: 44 us, with 256 blocks 54); in bf16, whose
+  // products take less time than its rows' loads, 256 (22 us, with 512 24).
   const bool small = M <= SMALL_ROWS, direct = M <= 1024;
   const long cols = 16 * (x.element_size() == 4 ? 4 : 8);
   const long chunks = (K + cols - 1) / cols;
+  const long wanted = x.scalar_type() == torch::kBFloat16 ? 256 : 512;
   const long stretch =
-      direct ? 1 : std::max<long>(4, M / TILE * chunks / 1024);
+      direct ? 1 : std::max<long>(4, M / TILE * chunks / wanted);
   const long slots = direct ? E : tiles / stretch + E;
   torch::Tensor partial;
   if (!direct)
@@ -947,7 +1248,7 @@ torch::Tensor adapter_outer(torch::Tensor x, torch::Tensor z,
       auto go = [&](auto kernel) {
         hipLaunchKernelGGL(
             kernel,
-            dim3((unsigned)slots, (unsigned)chunks,
+            dim3((unsigned)chunks, (unsigned)slots,
                  (unsigned)(padded_rank(R) / (16 * RB))),
             dim3(256), 0, stream, ptr<T>(x), (long)x.stride(0), zp,
             (int)z.size(1), p, ptr<T>(out),

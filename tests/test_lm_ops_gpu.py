@@ -458,20 +458,21 @@ def test_adapter_plan(m, e):
     ids = torch.randint(-2, e + 2, (m,), generator=gen)
     plan = ops.hip.adapter_plan(ids.to(DEV), e).cpu()
     group = torch.where(ids < 0, e, torch.where(ids >= e, e + 1, ids))
-    order = torch.sort(group, stable=True)[1]
-    assert torch.equal(plan[:m].long(), order)
-    counts = torch.bincount(group, minlength=e + 2)
-    seg, tbase = plan[m:m + e + 3], plan[m + e + 3:m + 2 * e + 6]
-    assert seg.tolist() == [0] + counts.cumsum(0).tolist()
-    tiles = (counts + 15) // 16
-    assert tbase.tolist() == [0] + tiles.cumsum(0).tolist()
-    most = m // 16 + min(e + 2, m)
-    of, place = plan[m + 2 * e + 6:].reshape(2, most)
-    n = int(tiles.sum())
-    want = [(g, int(seg[g]) + 16 * j) for g in range(e + 2)
-            for j in range(int(tiles[g]))]
-    assert list(zip(of[:n].tolist(), place[:n].tolist())) == want
-    assert (of[n:] == -1).all()
+    counts = torch.bincount(group, minlength=e + 2).tolist()
+    starts = [0] + torch.tensor(counts).cumsum(0).tolist()
+    sizes = []
+    for rows in (16, 64):  # tiles and blocks
+        most = m // rows + min(e + 2, m)
+        table, plan = plan[:4 * most].reshape(most, 4), plan[4 * most:]
+        want = [[g, starts[g] + at, min(rows, counts[g] - at), 0]
+                for g in range(e + 2) for at in range(0, counts[g], rows)]
+        assert table[:len(want)].tolist() == want
+        assert (table[len(want):, 0] == -1).all()
+        sizes.append([-(-c // rows) for c in counts])
+    perm, seg, tbase = plan.split([m, e + 3, e + 3])
+    assert torch.equal(perm.long(), torch.sort(group, stable=True)[1])
+    assert seg.tolist() == starts
+    assert tbase.tolist() == [0] + torch.tensor(sizes[0]).cumsum(0).tolist()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
