@@ -632,20 +632,14 @@ def _philox_words(state: torch.Tensor, n: int) -> torch.Tensor:
     return torch.stack((c0, c1, c2, c3), 1).reshape(-1)[:n]
 
 
-class Dropout(torch.autograd.Function):
+class _DropoutCPU(torch.autograd.Function):
     """The mask is a function of the state and the element's index; only
     the state is kept, and backward draws the same mask again."""
 
     @staticmethod
-    def forward(ctx, x, state, p: float):
+    def forward(ctx, x, state, keep: int, scale: float):
         ctx.save_for_backward(state)
-        ctx.p = p
-        keep = round((1.0 - p) * 2 ** 32)  # of 2^32 words
-        if keep == 0:
-            return torch.zeros_like(x, memory_format=torch.contiguous_format)
-        scale = 1.0 / (1.0 - p)
-        if ops.use_hip(x):
-            return ops.hip.dropout(x.contiguous(), state, keep, scale)
+        ctx.conf = (keep, scale)
         kept = (_philox_words(state, x.numel()) < keep).reshape(x.shape)
         y = (x.to(torch.float32) * scale).to(x.dtype)
         return torch.where(kept, y, torch.zeros_like(y))
@@ -653,7 +647,7 @@ class Dropout(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         (state,) = ctx.saved_tensors
-        return Dropout.apply(dy, state, ctx.p), None, None
+        return _DropoutCPU.apply(dy, state, *ctx.conf), None, None, None
 
 
 def dropout(x, p: float, state, training: bool = True):
@@ -675,7 +669,11 @@ def dropout(x, p: float, state, training: bool = True):
                          % (x.device, state.device))
     if not training or p == 0.0:
         return x
-    return Dropout.apply(x, state, float(p))
+    keep = round((1.0 - p) * 2 ** 32)  # of 2^32 words
+    scale = 1.0 / (1.0 - p) if keep else 0.0
+    if ops.use_hip(x):
+        return ops.hip.dropout_apply(x, state, keep, scale)
+    return _DropoutCPU.apply(x, state, keep, scale)
 
 
 # -- log-probabilities of given tokens ----------------------------------------
@@ -692,17 +690,13 @@ class TokenLogProbs(NamedTuple):
     top_ids: torch.Tensor
 
 
-class _TokenLogProbs(torch.autograd.Function):
+class _TokenLogProbsCPU(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, tokens, k: int, ignore: int):
         ctx.set_materialize_grads(False)
-        if ops.use_hip(logits):
-            logp, entropy, stat, top, ids = ops.hip.logprobs_fwd(
-                logits, tokens, k, ignore)
-        else:
-            logp, entropy, stat, top, ids = _logprobs_cpu(
-                logits, tokens.long(), k, ignore)
+        logp, entropy, stat, top, ids = _logprobs_cpu(logits, tokens, k,
+                                                      ignore)
         ctx.save_for_backward(logits, tokens, stat, entropy, ids)
         ctx.ignore = ignore
         ctx.mark_non_differentiable(ids)
@@ -711,15 +705,8 @@ class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_logp, g_entropy, g_top, _):
-        logits, tokens, stat, entropy, ids = ctx.saved_tensors
-        gs = [None if g is None else g.contiguous()
-              for g in (g_logp, g_entropy, g_top)]
-        if ops.use_hip(logits):
-            dx = ops.hip.logprobs_bwd(logits, tokens, stat, entropy, ids,
-                                      *gs, ctx.ignore)
-        else:
-            dx = _logprobs_grad_cpu(logits, tokens.long(), stat, entropy,
-                                    ids, *gs, ctx.ignore)
+        dx = _logprobs_grad_cpu(*ctx.saved_tensors, g_logp, g_entropy, g_top,
+                                ctx.ignore)
         return dx, None, None, None
 
 
@@ -831,15 +818,16 @@ def token_logprobs(logits, tokens, top_k: int = 0,
     if not 0 <= top_k <= min(_TOP_MAX, classes):
         raise ValueError("top_k must be within 0 and min(%d, %d classes), "
                          "got %r" % (_TOP_MAX, classes, top_k))
-    shape = tokens.shape
-    rows = logits.reshape(-1, classes)
-    if rows.stride(1) != 1 and classes > 1:
-        rows = rows.contiguous()
-    tokens = tokens.detach().reshape(-1)
-    if tokens.dtype != torch.float32:
+    tokens = tokens.detach()
+    if tokens.dtype not in (torch.float32, torch.int64):
         tokens = tokens.long()
-    logp, entropy, top, ids = _TokenLogProbs.apply(
-        rows, tokens.contiguous(), int(top_k), int(ignore_index))
+    if ops.use_hip(logits):
+        return TokenLogProbs(*ops.hip.logprobs_apply(
+            logits, tokens, top_k, ignore_index))
+    shape = tokens.shape
+    logp, entropy, top, ids = _TokenLogProbsCPU.apply(
+        logits.reshape(-1, classes), tokens.reshape(-1).long(), top_k,
+        ignore_index)
     return TokenLogProbs(logp.reshape(shape), entropy.reshape(shape),
                          top.reshape(shape + (top_k,)),
                          ids.reshape(shape + (top_k,)))
@@ -857,7 +845,8 @@ class AdapterGroups:
     def __init__(self, ids, adapters: int):
         self.adapters = adapters
         self.shape = ids.shape
-        self.ids = ids.detach().reshape(-1).long().contiguous()
+        # its own copy: what the caller does to ids later changes nothing
+        self.ids = ids.detach().reshape(-1).to(torch.int64, copy=True)
         self.device = ids.device
         self.plan = ops.hip.adapter_plan(self.ids, adapters) \
             if ops.use_hip(ids) else None
@@ -869,6 +858,11 @@ def adapter_groups(ids, adapters: int) -> AdapterGroups:
     ids: whole numbers in an integer type, one a row.  0 .. adapters - 1
     name an adapter, a negative number none.
     """
+    _check_ids(ids, adapters)
+    return AdapterGroups(ids, adapters)
+
+
+def _check_ids(ids, adapters: int) -> None:
     if ids.dtype == torch.bool or ids.is_floating_point() \
             or ids.is_complex():
         raise ValueError("ids must be whole numbers in an integer type, "
@@ -876,83 +870,56 @@ def adapter_groups(ids, adapters: int) -> AdapterGroups:
     if not 1 <= adapters <= _ADAPTERS_MAX:
         raise ValueError("adapters must be within 1 and %d, got %r"
                          % (_ADAPTERS_MAX, adapters))
-    return AdapterGroups(ids, adapters)
 
 
-class _AdapterAdd(torch.autograd.Function):
+class _AdapterAddCPU(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, base, x, a, b, scales, scale, groups, act: int):
-        if ops.use_hip(x):
-            z = ops.hip.adapter_shrink(x, a, groups.ids, groups.plan, scales, scale,
-                                       True)
-            y = ops.hip.adapter_expand(base, z, b, groups.ids, groups.plan, act, True)
-        else:
-            z, y = _adapter_cpu(base, x, a, b, scales, scale, groups, act)
-        ctx.save_for_backward(x, a, b, z, scales,
+    def forward(ctx, base, x, a, b, scales, scale, ids, act: int):
+        z, y = _adapter_cpu(base, x, a, b, scales, scale, ids, act)
+        ctx.save_for_backward(x, a, b, z, scales, ids,
                               y if act != ACT_NONE else None)
-        ctx.conf = (scale, groups, act)
+        ctx.conf = (scale, act)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, a, b, z, scales, y = ctx.saved_tensors
-        scale, groups, act = ctx.conf
-        need_base, need_x, need_a, need_b = ctx.needs_input_grad[:4]
-        e, r, _ = a.shape
-        dy = dy.contiguous()
-        if not ops.use_hip(x):
-            grads = _adapter_grad_cpu(x, a, b, z, scales, y, dy, scale,
-                                      groups, act)
-            return tuple(g if need else None for g, need in zip(
-                grads, ctx.needs_input_grad)) + (None,) * 4
-        if act != ACT_NONE:
-            dy = ops.hip.adapter_act_bwd(y, dy, act)
-        dx = da = db = None
-        if need_x or need_a:
-            dz = ops.hip.adapter_shrink(dy, b, groups.ids, groups.plan, scales, scale,
-                                        False)
-        if need_x:
-            dx = ops.hip.adapter_expand(None, dz, a, groups.ids, groups.plan, ACT_NONE,
-                                        False)
-        if need_a:
-            da = ops.hip.adapter_outer(x, dz, groups.ids, groups.plan, e, r, True)
-        if need_b:
-            db = ops.hip.adapter_outer(dy, z, groups.ids, groups.plan, e, r, False)
-        return (dy if need_base else None, dx, da, db) + (None,) * 4
+        grads = _adapter_grad_cpu(*ctx.saved_tensors, dy, *ctx.conf)
+        return tuple(g if need else None for g, need in zip(
+            grads, ctx.needs_input_grad)) + (None,) * 4
 
 
-def _adapter_rows(groups, scales, scale):
-    for e in range(groups.adapters):
-        rows = (groups.ids == e).nonzero().squeeze(1)
+def _adapter_rows(ids, adapters, scales, scale):
+    for e in range(adapters):
+        rows = (ids == e).nonzero().squeeze(1)
         if len(rows):
             yield e, rows, scale if scales is None else scales[e]
 
 
-def _adapter_cpu(base, x, a, b, scales, scale, groups, act):
+def _adapter_cpu(base, x, a, b, scales, scale, ids, act):
     f32 = torch.float32
     y = base.to(f32).clone()
     z = torch.zeros(x.shape[0], a.shape[1])
-    for e, rows, s in _adapter_rows(groups, scales, scale):
+    for e, rows, s in _adapter_rows(ids, len(a), scales, scale):
         z[rows] = s * (x[rows].to(f32) @ a[e].to(f32).t())
         y[rows] += z[rows] @ b[e].to(f32).t()
-    y[groups.ids >= groups.adapters] = float("nan")
+    y[ids >= len(a)] = float("nan")
     return z, _act_fwd(y, act).to(base.dtype)
 
 
-def _adapter_grad_cpu(x, a, b, z, scales, y, dy, scale, groups, act):
+def _adapter_grad_cpu(x, a, b, z, scales, ids, y, dy, scale, act):
     f32 = torch.float32
     if act != ACT_NONE:
         dy = _act_bwd_from_out(y.to(f32), dy.to(f32), act).to(dy.dtype)
     dx, da, db = (torch.zeros(t.shape) for t in (x, a, b))
-    for e, rows, s in _adapter_rows(groups, scales, scale):
+    for e, rows, s in _adapter_rows(ids, len(a), scales, scale):
         g = dy[rows].to(f32)
         dz = s * (g @ b[e].to(f32))
         dx[rows] = dz @ a[e].to(f32)
         da[e] = dz.t() @ x[rows].to(f32)
         db[e] = g.t() @ z[rows]
-    dx[groups.ids >= groups.adapters] = float("nan")
+    dx[ids >= len(a)] = float("nan")
     return dy, dx.to(x.dtype), da.to(a.dtype), db.to(b.dtype)
 
 
@@ -1012,19 +979,24 @@ def adapter_add(base, x, a, b, ids, scale=1.0, act="none"):
             raise ValueError("scale must be a number, or fp32 [%d] beside x"
                              % e)
         scales, scale = scale.contiguous(), 1.0
+    else:
+        scale = float(scale)
+    plan = None
     if groups is None:
-        groups = adapter_groups(ids, e)
+        _check_ids(ids, e)
+        if ids.dtype != torch.int64:
+            ids = ids.long()
     elif groups.adapters != e:
         raise ValueError("ids were grouped for %d adapters, not %d"
                          % (groups.adapters, e))
-
-    def rows(t, width):
-        t = t.reshape(-1, width)
-        return t if t.stride(1) == 1 or width == 1 else t.contiguous()
-
-    y = _AdapterAdd.apply(rows(base, n), rows(x, k), a.contiguous(),
-                          b.contiguous(), scales, float(scale), groups, act)
-    return y.reshape(base.shape)
+    else:
+        ids, plan = groups.ids, groups.plan
+    if ops.use_hip(x):
+        return ops.hip.adapter_add_apply(base, x, a, b, scales, scale, ids,
+                                         plan, act)
+    return _AdapterAddCPU.apply(
+        base.reshape(-1, n), x.reshape(-1, k), a, b, scales, scale,
+        ids.reshape(-1), act).reshape(base.shape)
 
 
 def argmax_rows(y: torch.Tensor) -> torch.Tensor:

@@ -3,6 +3,8 @@
 
 #include <vector>
 
+#include "lm_ops.h"
+
 // gemm.hip
 torch::Tensor gemm_act(torch::Tensor x, torch::Tensor w, torch::Tensor bias,
                        int64_t act);
@@ -45,39 +47,6 @@ torch::Tensor mse_fwd(torch::Tensor pred, torch::Tensor target,
                       bool want_value);
 torch::Tensor mse_bwd(torch::Tensor pred, torch::Tensor target,
                       torch::Tensor gscale, double mult);
-
-// dropout.hip — mask drawn from a counter, never stored
-torch::Tensor dropout(torch::Tensor x, torch::Tensor state, int64_t keep,
-                      double scale);
-torch::Tensor dropout_next(torch::Tensor state);
-
-// logprobs.hip — scores of given tokens, entropy, best alternatives
-std::vector<torch::Tensor> logprobs_fwd(torch::Tensor logits,
-                                        torch::Tensor tokens, int64_t k,
-                                        int64_t ignore);
-torch::Tensor logprobs_bwd(torch::Tensor logits, torch::Tensor tokens,
-                           torch::Tensor stat, torch::Tensor entropy,
-                           torch::Tensor ids,
-                           c10::optional<torch::Tensor> g_logp,
-                           c10::optional<torch::Tensor> g_entropy,
-                           c10::optional<torch::Tensor> g_top,
-                           int64_t ignore);
-
-// adapter.hip — low-rank adapters of many requests
-torch::Tensor adapter_plan(torch::Tensor ids, int64_t E);
-torch::Tensor adapter_shrink(torch::Tensor x, torch::Tensor w,
-                             torch::Tensor ids, torch::Tensor plan,
-                             c10::optional<torch::Tensor> scales,
-                             double scale, bool kmajor);
-torch::Tensor adapter_expand(c10::optional<torch::Tensor> base,
-                             torch::Tensor z, torch::Tensor w,
-                             torch::Tensor ids, torch::Tensor plan,
-                             int64_t act, bool rmajor);
-torch::Tensor adapter_outer(torch::Tensor x, torch::Tensor z,
-                            torch::Tensor ids, torch::Tensor plan, int64_t E,
-                            int64_t R, bool kmajor);
-torch::Tensor adapter_act_bwd(torch::Tensor y, torch::Tensor dy,
-                              int64_t act);
 
 // optim.hip
 void fused_sgd(torch::Tensor p, torch::Tensor g, double lr);
@@ -216,33 +185,22 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mse_fwd", &mse_fwd, "fused MSE loss", py::arg("pred"),
         py::arg("target"), py::arg("want_value") = true);
   m.def("mse_bwd", &mse_bwd, "MSE grad");
-  m.def("dropout", &dropout,
-        "dropout by Philox4x32-10 of (seed, offset, element); its own "
-        "backward");
+  m.def("dropout_apply", &dropout_apply,
+        "dropout by Philox4x32-10 of (seed, offset, element), with its "
+        "gradient");
   m.def("dropout_next", &dropout_next,
         "the state of one draw; steps the given state on in place");
-  m.def("logprobs_fwd", &logprobs_fwd,
-        "token log-probs + row entropy + top-k; one read of logits");
-  m.def("logprobs_bwd", &logprobs_bwd,
-        "dlogits from the gradients of log-probs, entropy and top-k",
-        py::arg("logits"), py::arg("tokens"), py::arg("stat"),
-        py::arg("entropy"), py::arg("ids"), py::arg("g_logp") = py::none(),
-        py::arg("g_entropy") = py::none(), py::arg("g_top") = py::none(),
-        py::arg("ignore") = -100);
+  m.def("logprobs_apply", &logprobs_apply,
+        "token log-probs, row entropy and top-k from one read of the "
+        "logits, with their gradients");
   m.def("adapter_plan", &adapter_plan,
-        "rows grouped by adapter: order, groups and tiles of 16 rows");
-  m.def("adapter_shrink", &adapter_shrink,
-        "z = scale * x w^T by adapter, fp32, in grouped order",
-        py::arg("x"), py::arg("w"), py::arg("ids"), py::arg("plan"),
-        py::arg("scales"), py::arg("scale"), py::arg("kmajor"));
-  m.def("adapter_expand", &adapter_expand,
-        "act(base + z w^T) by adapter", py::arg("base"), py::arg("z"),
-        py::arg("w"), py::arg("ids"), py::arg("plan"), py::arg("act"),
-        py::arg("rmajor"));
-  m.def("adapter_outer", &adapter_outer,
-        "sums of z^T x over each adapter's rows");
-  m.def("adapter_act_bwd", &adapter_act_bwd,
-        "activation backward from output, fp32 / bf16 / fp16");
+        "rows grouped by adapter: order, groups, tiles of 16 rows and "
+        "blocks of 64");
+  m.def("adapter_add_apply", &adapter_add_apply,
+        "act(base + scale * (x a^T) b^T) by adapter, with its gradients",
+        py::arg("base"), py::arg("x"), py::arg("a"), py::arg("b"),
+        py::arg("scales"), py::arg("scale"), py::arg("ids"),
+        py::arg("plan"), py::arg("act"));
   m.def("fused_sgd", &fused_sgd, "single-launch SGD apply");
   m.def("fused_momentum", &fused_momentum, "single-launch momentum apply");
   m.def("fused_adam", &fused_adam, "single-launch Adam apply");

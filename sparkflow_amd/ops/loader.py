@@ -28,6 +28,7 @@ SOURCES = [
     HERE / "hip" / "dropout.hip",
     HERE / "hip" / "logprobs.hip",
     HERE / "hip" / "adapter.hip",
+    HERE / "hip" / "lm_autograd.cpp",
 ]
 
 # Packed fp32 instructions (v_pk_add/mul/fma_f32) stay out of every kernel:
