@@ -12,10 +12,10 @@
 //
 // Forward reads the logits once: every thread keeps its own (m, s, t), a
 // block joins them, and a row may be split over blocks that a second kernel
-// joins.  The alternatives need no second pass over the row: a thread's
-// maximum orders the threads, and with (value, lowest index) as the order
-// the k best elements of a block all lie with the k threads whose maxima are
-// largest, so only those k threads' elements are read again.
+// joins.  The alternatives need no second pass over the row: of 64 groups
+// of threads, the k-th largest maximum is a value that k elements reach, so
+// only the threads whose own maximum reaches it, hardly more than k, read
+// their elements again.
 //
 // All sums and statistics are fp32; outputs are fp32.
 #include <torch/extension.h>
@@ -47,14 +47,19 @@ __device__ __forceinline__ Stat stat_join(Stat a, Stat b) {
   return {m, a.s + b.s, a.t + b.t};
 }
 
-// An element in the order of the alternatives: larger values first, equal
-// values (both zeros among them) by the lower index.  0 is no element; a
-// NaN is none either, since its row has no alternatives.
-__device__ __forceinline__ unsigned long order_key(float x, unsigned idx) {
-  if (x != x) return 0;
+// A value in an order that whole numbers keep; both zeros are one.  0 is
+// below every number and stands for NaN, whose row has no alternatives.
+__device__ __forceinline__ unsigned order_of(float x) {
   const unsigned b = __float_as_uint(x + 0.0f);
-  const unsigned o = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-  return ((unsigned long)o << 32) | (0xFFFFFFFFu - idx);
+  if (x != x) return 0;
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
+// An element in the order of the alternatives: larger values first, equal
+// ones by the lower index.  0 is no element.
+__device__ __forceinline__ unsigned long order_key(unsigned order,
+                                                   unsigned idx) {
+  return order ? ((unsigned long)order << 32) | (0xFFFFFFFFu - idx) : 0;
 }
 
 __device__ __forceinline__ float key_value(unsigned long key) {
@@ -71,11 +76,28 @@ __device__ __forceinline__ unsigned long key_max(unsigned long a,
   return a > b ? a : b;
 }
 
-__device__ __forceinline__ unsigned long wave_key_max(unsigned long v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1)
-    v = key_max(v, __shfl_xor(v, off, WAVE));
-  return v;
+// The wave's largest, in every lane: six steps within the vector unit, where
+// a shuffle goes through LDS.
+__device__ __forceinline__ unsigned wave_max_u32(unsigned v) {
+#define STEP(ctrl, rows)                                                    \
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows,   \
+                                                   0xf, false))
+  STEP(0x111, 0xf);  // from one lane lower, of 16
+  STEP(0x112, 0xf);
+  STEP(0x114, 0xf);
+  STEP(0x118, 0xf);
+  STEP(0x142, 0xa);  // the last of 16 to the next 16
+  STEP(0x143, 0xc);  // the last of 32 to the next 32
+#undef STEP
+  return (unsigned)__builtin_amdgcn_readlane((int)v, WAVE - 1);
+}
+
+// The same of keys: the larger halves first, then the others among equals.
+__device__ __forceinline__ unsigned long wave_key_max(unsigned long key) {
+  const unsigned high = (unsigned)(key >> 32);
+  const unsigned top = wave_max_u32(high);
+  const unsigned low = wave_max_u32(high == top ? (unsigned)key : 0);
+  return ((unsigned long)top << 32) | low;
 }
 
 // Labels are int64, or fp32 that hold whole numbers (the engine's labels).
@@ -145,9 +167,9 @@ __device__ __forceinline__ void write_top(const RowOut& o, long row, int k,
   o.ids[row * k + j] = id;
 }
 
-// One block per (row, split).  NT threads; thread t owns the vectors
-// t, t + NT, t + 2 NT ... of the split and, if it is the last thread, the
-// elements behind the last whole vector.
+// One block per (row, split).  Thread t of NT owns the vectors t, t + NT,
+// t + 2 NT ... of the split and, if it is the last thread, the elements
+// behind the last whole vector.
 template <typename T, int NT, int UNROLL, bool TOP>
 __global__ void __launch_bounds__(NT)
     logprobs_fwd_kernel(const T* __restrict__ logits, long stride,
@@ -156,12 +178,13 @@ __global__ void __launch_bounds__(NT)
                         long span, int k) {
   constexpr int N = Vec<T>::N;
   constexpr int CAP = 512;
+  typedef typename Vec<T>::V V;
   __shared__ Stat wstat[NT / WAVE];
-  __shared__ __attribute__((aligned(16))) unsigned long keys[TOP ? NT : 2];
+  __shared__ __attribute__((aligned(16))) unsigned groups[WAVE];
   __shared__ unsigned long cand[TOP ? CAP : 1];
-  __shared__ int owners[TOP_MAX];
-  __shared__ int count;
-  __shared__ unsigned long bar;
+  __shared__ int owners[NT];
+  __shared__ unsigned bar;
+  __shared__ int nown, count;
 
   const int tid = threadIdx.x;
   const int lane = tid & (WAVE - 1), wave = tid / WAVE;
@@ -175,69 +198,92 @@ __global__ void __launch_bounds__(NT)
   const T* xr = logits + row * stride;
   const long lo = split * span;
   const long hi = lo + span < C ? lo + span : C;
+  const T* part = xr + lo;
   const int vecs = (int)((hi - lo) / N);  // whole vectors
   const int tail = (int)((hi - lo) % N);
 
-  // -- one pass: (m, s, t) and where m came from
+  // -- one pass: (m, s, t), the sums in two halves for shorter chains
   Stat a = {-INFINITY, 0.0f, 0.0f};
-  int from = tid;  // the vector, of this thread's, that raised m last
-  for (int v0 = tid; v0 < vecs; v0 += NT * UNROLL) {
-    typename Vec<T>::V v[UNROLL];
-    float x[UNROLL][N];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
-      if (v0 + u * NT < vecs)
-        v[u] = Vec<T>::load(xr + lo + (long)(v0 + u * NT) * N);
+  float s1 = 0.0f, t1 = 0.0f;
+  auto take = [&](const float* x, int n) {
     float gm = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const bool in = v0 + u * NT < vecs;
+    for (int j = 0; j < n; ++j) gm = fmaxf(gm, x[j]);
+    if (gm > a.m) {  // seldom, but at the start
+      const Stat b = stat_at({a.m, s1, t1}, gm);
+      a = stat_at(a, gm);
+      s1 = b.s;
+      t1 = b.t;
+    }
+    if (a.m == -INFINITY) {  // nothing but -inf so far, and perhaps NaN
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        x[u][j] = in ? (float)v[u][j] : -INFINITY;
-        gm = fmaxf(gm, x[u][j]);
+      for (int j = 0; j < n; ++j)
+        if (x[j] != x[j]) a.s = x[j];
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < n; ++j) {
+      const float d = x[j] - a.m;
+      const float e = __expf(d);
+      // -inf: e is 0 and must meet a finite factor
+      const float f = fmaxf(d, -1000.0f);
+      if (j % 2 == 0) {
+        a.s += e;
+        a.t = fmaf(e, f, a.t);
+      } else {
+        s1 += e;
+        t1 = fmaf(e, f, t1);
       }
     }
-    if (gm > a.m) {
-      a = stat_at(a, gm);
-      if (TOP) from = v0;
-    }
-    if (a.m == -INFINITY) {
-      // nothing but -inf so far, and perhaps NaN
+  };
+  // whole rounds of the block without a branch, the next one's loads under
+  // way; then what is left
+  constexpr int ROUND = NT * UNROLL;
+  const int rounds = vecs / ROUND;
+  V v[UNROLL];
+  auto load = [&](int r) {
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u)
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (x[u][j] != x[u][j]) a.s = x[u][j];
-      continue;
-    }
+    for (int u = 0; u < UNROLL; ++u)
+      v[u] = Vec<T>::load(part + (long)(r * ROUND + u * NT + tid) * N);
+  };
+  if (rounds > 0) load(0);
+  for (int r = 0; r < rounds; ++r) {
+    float x[UNROLL * N];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float d = x[u][j] - a.m;
-        const float e = __expf(d);
-        a.s += e;
-        // -inf: e is 0 and must meet a finite factor
-        a.t = fmaf(e, fmaxf(d, -1000.0f), a.t);
-      }
+      for (int j = 0; j < N; ++j) x[u * N + j] = (float)v[u][j];
+    if (r + 1 < rounds) load(r + 1);
+    take(x, UNROLL * N);
   }
-  bool from_tail = false;
-  if (tid == NT - 1) {
+  for (int at = rounds * ROUND + tid; at < vecs; at += NT) {
+    const V w = Vec<T>::load(part + (long)at * N);
+    float x[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = (float)w[j];
+    take(x, N);
+  }
+  if (tid == NT - 1)
     for (int j = 0; j < tail; ++j) {
-      const float x = (float)xr[lo + (long)vecs * N + j];
-      if (x > a.m) {
-        a = stat_at(a, x);
-        from_tail = true;
-      }
-      if (a.m == -INFINITY) {
-        if (x != x) a.s = x;
-        continue;
-      }
-      const float d = x - a.m;
-      const float e = __expf(d);
-      a.s += e;
-      a.t = fmaf(e, fmaxf(d, -1000.0f), a.t);
+      const float x = (float)part[(long)vecs * N + j];
+      take(&x, 1);
+    }
+  a.s += s1;
+  a.t += t1;
+
+  // the thread's maximum, and that of its group
+  const bool any = tid < vecs || (tid == NT - 1 && tail > 0);
+  const unsigned own = any ? order_of(a.m) : 0;
+  if (TOP) {
+    constexpr int G = NT / WAVE;  // threads of a group: 1 or 4
+    unsigned g = own;
+#pragma unroll
+    for (int off = 1; off < G; off <<= 1)
+      g = max(g, (unsigned)__shfl_xor((int)g, off, WAVE));
+    if (tid % G == 0) groups[tid / G] = g;
+    if (tid == 0) {
+      bar = 0xFFFFFFFFu;
+      nown = count = 0;
     }
   }
 
@@ -246,13 +292,11 @@ __global__ void __launch_bounds__(NT)
   for (int off = 32; off > 0; off >>= 1)
     a = stat_join(a, {__shfl_xor(a.m, off, WAVE), __shfl_xor(a.s, off, WAVE),
                       __shfl_xor(a.t, off, WAVE)});
-  if (NT > WAVE) {
-    if (lane == 0) wstat[wave] = a;
-    __syncthreads();
-    a = wstat[0];
+  if (lane == 0) wstat[wave] = a;
+  __syncthreads();
+  a = wstat[0];
 #pragma unroll
-    for (int w = 1; w < NT / WAVE; ++w) a = stat_join(a, wstat[w]);
-  }
+  for (int w = 1; w < NT / WAVE; ++w) a = stat_join(a, wstat[w]);
   if (tid == 0) {
     if (splits == 1) {
       write_stats(out, row, a, xr, C, token);
@@ -265,67 +309,46 @@ __global__ void __launch_bounds__(NT)
   }
   if (!TOP) return;
 
-  // -- the thread's own best element, by reading its vectors again
-  unsigned long best = 0;
-  if (tid < vecs) {
+  // -- the bar: the smallest of the groups' k largest maxima (0, which
+  // every element reaches, if there are not k groups that hold anything)
+  if (wave == 0) {
+    const unsigned mine = groups[lane];
+    int above = 0;
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int at = from + u * NT;
-      if (at >= vecs) break;
-      const typename Vec<T>::V v = Vec<T>::load(xr + lo + (long)at * N);
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        best = key_max(best,
-                       order_key((float)v[j], (unsigned)(lo + (long)at * N + j)));
+    for (int i = 0; i < WAVE; i += 4) {
+      const uint4 g = *reinterpret_cast<const uint4*>(&groups[i]);
+      above += (g.x > mine) + (g.y > mine) + (g.z > mine) + (g.w > mine);
     }
-  }
-  if (tid == NT - 1 && (from_tail || tid >= vecs)) {
-    for (int j = 0; j < tail; ++j)
-      best = key_max(best, order_key((float)xr[lo + (long)vecs * N + j],
-                                     (unsigned)(lo + (long)vecs * N + j)));
-  }
-  keys[tid] = best;
-  if (tid == 0) {
-    count = 0;
-    bar = 0;
+    if (above < k) atomicMin(&bar, mine);
   }
   __syncthreads();
-  int rank = 0;
-  for (int i = 0; i < NT; ++i) rank += keys[i] > best ? 1 : 0;
-  if (best != 0 && rank < k) {
-    owners[rank] = tid;
-    atomicAdd(&count, 1);
-    if (rank == k - 1) bar = best;
-  }
-  __syncthreads();
-  const int nown = count;  // threads that own anything, at most k
-  const unsigned long floor_key = bar;
-  __syncthreads();
-  if (tid == 0) count = 0;
+  const unsigned least = max(bar, 1u);
+  if (own >= least) owners[atomicAdd(&nown, 1)] = tid;
   __syncthreads();
 
-  // -- the elements of those threads that reach the k-th best maximum
+  // -- every element that reaches it, from the threads that have one
+  const int n_own = nown;
   const int per = (vecs + NT - 1) / NT;  // vectors of one thread, at most
-  for (int w = tid; w < nown * per; w += NT) {
+  for (int w = tid; w < n_own * per; w += NT) {
     const int at = owners[w / per] + (w % per) * NT;
     if (at >= vecs) continue;
-    const typename Vec<T>::V v = Vec<T>::load(xr + lo + (long)at * N);
+    const V x = Vec<T>::load(part + (long)at * N);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const unsigned long key =
-          order_key((float)v[j], (unsigned)(lo + (long)at * N + j));
-      if (key != 0 && key >= floor_key) {
+      const unsigned o = order_of((float)x[j]);
+      if (o >= least) {
         const int i = atomicAdd(&count, 1);
-        if (i < CAP) cand[i] = key;
+        if (i < CAP)
+          cand[i] = order_key(o, (unsigned)(lo + (long)at * N + j));
       }
     }
   }
-  for (int j = tid; j < tail; j += NT) {
-    const unsigned long key = order_key((float)xr[lo + (long)vecs * N + j],
-                                        (unsigned)(lo + (long)vecs * N + j));
-    if (key != 0 && key >= floor_key) {
+  if (tid < tail) {
+    const unsigned o = order_of((float)part[(long)vecs * N + tid]);
+    if (o >= least) {
       const int i = atomicAdd(&count, 1);
-      if (i < CAP) cand[i] = key;
+      if (i < CAP)
+        cand[i] = order_key(o, (unsigned)(lo + (long)vecs * N + tid));
     }
   }
   __syncthreads();
@@ -348,30 +371,32 @@ __global__ void __launch_bounds__(NT)
     for (int j = n + tid; j < k; j += NT) emit(j, 0);
     return;
   }
-  // More candidates than the list holds: large values that sit together in
-  // few threads' vectors.  Take them one after another, the largest below
+  // More than the list holds: many equal values, or the large ones together
+  // in few threads' vectors.  Take them one after another, the largest below
   // the last.
   unsigned long last = ~0ul;
   for (int j = 0; j < k; ++j) {
     unsigned long top = 0;
-    for (int w = tid; w < nown * per; w += NT) {
+    for (int w = tid; w < n_own * per; w += NT) {
       const int at = owners[w / per] + (w % per) * NT;
       if (at >= vecs) continue;
-      const typename Vec<T>::V v = Vec<T>::load(xr + lo + (long)at * N);
+      const V x = Vec<T>::load(part + (long)at * N);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const unsigned long key =
-            order_key((float)v[i], (unsigned)(lo + (long)at * N + i));
+            order_key(order_of((float)x[i]),
+                      (unsigned)(lo + (long)at * N + i));
         if (key < last) top = key_max(top, key);
       }
     }
-    for (int i = tid; i < tail; i += NT) {
-      const unsigned long key = order_key((float)xr[lo + (long)vecs * N + i],
-                                          (unsigned)(lo + (long)vecs * N + i));
+    if (tid < tail) {
+      const unsigned long key =
+          order_key(order_of((float)part[(long)vecs * N + tid]),
+                    (unsigned)(lo + (long)vecs * N + tid));
       if (key < last) top = key_max(top, key);
     }
     top = wave_key_max(top);
-    __syncthreads();  // the list, or the last round's maxima, were read
+    __syncthreads();  // the list, or the last turn's maxima, were read
     if (lane == 0) cand[wave] = top;
     __syncthreads();
 #pragma unroll
@@ -381,22 +406,27 @@ __global__ void __launch_bounds__(NT)
   }
 }
 
-// Joins the splits of a row, one wave a row.  Lane l holds split l.
+#define SPLITS_MAX 64
+
+// Joins the splits of a row, one wave a row.  Lane l holds split l and its
+// sorted list, which waits in LDS; the largest head is taken k times.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(WAVE)
     logprobs_join_kernel(const T* __restrict__ logits, long stride,
                          Tokens tokens, RowOut out,
                          const float* __restrict__ pstat,
-                         const unsigned long* __restrict__ pkeys, long M,
-                         long C, int splits, int k) {
-  const long row = (long)blockIdx.x * (256 / WAVE) + threadIdx.x / WAVE;
-  const int lane = threadIdx.x & (WAVE - 1);
-  if (row >= M) return;
+                         const unsigned long* __restrict__ pkeys, long C,
+                         int splits, int k) {
+  __shared__ unsigned long list[SPLITS_MAX * TOP_MAX];
+  const long row = blockIdx.x;
+  const int lane = threadIdx.x;
   const long token = token_of(tokens, row);
   if (token == tokens.ignore) {
     write_ignored(out, row, k, lane, WAVE);
     return;
   }
+  for (int i = lane; i < splits * k; i += WAVE)
+    list[i] = pkeys[row * splits * k + i];
   Stat a = {-INFINITY, 0.0f, 0.0f};
   if (lane < splits) {
     const float* p = pstat + (row * splits + lane) * 3;
@@ -407,18 +437,20 @@ __global__ void __launch_bounds__(256)
     a = stat_join(a, {__shfl_xor(a.m, off, WAVE), __shfl_xor(a.s, off, WAVE),
                       __shfl_xor(a.t, off, WAVE)});
   if (lane == 0) write_stats(out, row, a, logits + row * stride, C, token);
-  // every split's list is sorted: take the largest head k times
-  const unsigned long* list = pkeys + (row * splits + lane) * k;
+  if (k == 0) return;
+  __syncthreads();
   int at = 0;
-  unsigned long head = lane < splits && k > 0 ? list[0] : 0;
+  unsigned long head = lane < splits ? list[lane * k] : 0;
+  unsigned long mine = 0;  // lane j keeps the j-th
   for (int j = 0; j < k; ++j) {
     const unsigned long top = wave_key_max(head);
-    if (lane == 0) write_top(out, row, k, j, top, a);
-    if (top != 0 && head == top) {
+    if (lane == j) mine = top;
+    if (head == top && top != 0) {
       ++at;
-      head = at < k ? list[at] : 0;
+      head = at < k ? list[lane * k + at] : 0;
     }
   }
+  if (lane < k) write_top(out, row, k, lane, mine, a);
 }
 
 struct RowGrad {
@@ -566,8 +598,9 @@ std::vector<torch::Tensor> logprobs_fwd(torch::Tensor logits,
     // Split rows until the blocks fill the 256 CUs twice, in spans of
     // 4096 elements at least.
     long splits = 1;
-    if (M < 512) splits = std::min<long>(64, std::min((512 + M - 1) / M,
-                                                      (C + 4095) / 4096));
+    if (M < 512)
+      splits = std::min<long>(SPLITS_MAX, std::min((512 + M - 1) / M,
+                                                   (C + 4095) / 4096));
     long span = (C + splits - 1) / splits;
     span = (span + N - 1) / N * N;
     splits = (C + span - 1) / span;
@@ -595,15 +628,15 @@ std::vector<torch::Tensor> logprobs_fwd(torch::Tensor logits,
       else
         go(logprobs_fwd_kernel<T, 64, 1, false>, 64);
     } else if (k) {
-      go(logprobs_fwd_kernel<T, 256, 2, true>, 256);
+      go(logprobs_fwd_kernel<T, 256, 16 / N, true>, 256);
     } else {
-      go(logprobs_fwd_kernel<T, 256, 2, false>, 256);
+      go(logprobs_fwd_kernel<T, 256, 16 / N, false>, 256);
     }
     LAUNCH_OK();
     if (splits > 1) {
       hipLaunchKernelGGL((logprobs_join_kernel<T>),
-                         dim3((unsigned)((M + 3) / 4)), dim3(256), 0, stream,
-                         x, (long)logits.stride(0), tok, out, ps, pk, M, C,
+                         dim3((unsigned)M), dim3(WAVE), 0, stream, x,
+                         (long)logits.stride(0), tok, out, ps, pk, C,
                          (int)splits, (int)k);
       LAUNCH_OK();
     }
