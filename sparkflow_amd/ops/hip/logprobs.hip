@@ -55,6 +55,81 @@ __device__ __forceinline__ unsigned order_of(float x) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
+// A thread's own running sums, in steps of log 2 and about a whole number of
+// them: e^x / 2^shift is one exponential of one fused product, with one
+// rounding less than e^(x - m), and two instructions less an element, which
+// is what bounds the pass in the 16-bit types.  Two sums each, for shorter
+// chains.  Where m log2 e leaves fp32 (the lowest value as a mask of a whole
+// row) or is infinite, the sums are about m itself.
+struct Run {
+  float m, shift, s0, s1, t0, t1;
+
+  __device__ __forceinline__ bool far() const {
+    return !(fabsf(m) < 1.0e38f);
+  }
+
+  // Adds n values.
+  template <int n>
+  __device__ __forceinline__ void take(const float (&x)[n]) {
+    constexpr float LOG2E = 1.44269504089f;
+    float gm = x[0];
+#pragma unroll
+    for (int j = 1; j < n; ++j) gm = fmaxf(gm, x[j]);
+    if (gm > m) {  // seldom, but at the start
+      const Run old = *this;
+      m = gm;
+      shift = rintf(gm * LOG2E);
+      if (old.m != -INFINITY) {
+        const float d = far() || old.far() ? (old.m - m) * LOG2E
+                                           : old.shift - shift;
+        const float f = __builtin_amdgcn_exp2f(d);
+        // a maximum of infinite distance leaves nothing of the old sums
+        const float g = fmaxf(d, -1000.0f);
+        s0 = old.s0 * f;
+        s1 = old.s1 * f;
+        t0 = (old.t0 + old.s0 * g) * f;
+        t1 = (old.t1 + old.s1 * g) * f;
+      }
+    }
+    if (far()) {
+#pragma unroll
+      for (int j = 0; j < n; ++j) {
+        // nothing but -inf so far: only a NaN says anything
+        const float d = m == -INFINITY ? (x[j] != x[j] ? x[j] : -INFINITY)
+                                       : (x[j] - m) * LOG2E;
+        const float e = __builtin_amdgcn_exp2f(d);
+        s0 += e;
+        t0 = fmaf(e, fmaxf(d, -1000.0f), t0);
+      }
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < n; ++j) {
+      const float d = fmaf(x[j], LOG2E, -shift);
+      const float e = __builtin_amdgcn_exp2f(d);
+      // -inf: e is 0 and must meet a finite factor
+      const float f = fmaxf(d, -1000.0f);
+      if (j % 2 == 0) {
+        s0 += e;
+        t0 = fmaf(e, f, t0);
+      } else {
+        s1 += e;
+        t1 = fmaf(e, f, t1);
+      }
+    }
+  }
+
+  // The same about m, in natural steps.
+  __device__ __forceinline__ Stat stat() const {
+    constexpr float LOG2E = 1.44269504089f, LN2 = 0.69314718056f;
+    const float s = s0 + s1, t = t0 + t1;
+    if (far()) return {m, s, t * LN2};
+    const float d = fmaf(m, LOG2E, -shift);
+    const float f = __builtin_amdgcn_exp2f(-d);
+    return {m, s * f, (t - s * d) * f * LN2};
+  }
+};
+
 // An element in the order of the alternatives: larger values first, equal
 // ones by the lower index.  0 is no element.
 __device__ __forceinline__ unsigned long order_key(unsigned order,
@@ -202,40 +277,8 @@ __global__ void __launch_bounds__(NT)
   const int vecs = (int)((hi - lo) / N);  // whole vectors
   const int tail = (int)((hi - lo) % N);
 
-  // -- one pass: (m, s, t), the sums in two halves for shorter chains
-  Stat a = {-INFINITY, 0.0f, 0.0f};
-  float s1 = 0.0f, t1 = 0.0f;
-  auto take = [&](const float* x, int n) {
-    float gm = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < n; ++j) gm = fmaxf(gm, x[j]);
-    if (gm > a.m) {  // seldom, but at the start
-      const Stat b = stat_at({a.m, s1, t1}, gm);
-      a = stat_at(a, gm);
-      s1 = b.s;
-      t1 = b.t;
-    }
-    if (a.m == -INFINITY) {  // nothing but -inf so far, and perhaps NaN
-#pragma unroll
-      for (int j = 0; j < n; ++j)
-        if (x[j] != x[j]) a.s = x[j];
-      return;
-    }
-#pragma unroll
-    for (int j = 0; j < n; ++j) {
-      const float d = x[j] - a.m;
-      const float e = __expf(d);
-      // -inf: e is 0 and must meet a finite factor
-      const float f = fmaxf(d, -1000.0f);
-      if (j % 2 == 0) {
-        a.s += e;
-        a.t = fmaf(e, f, a.t);
-      } else {
-        s1 += e;
-        t1 = fmaf(e, f, t1);
-      }
-    }
-  };
+  // -- one pass
+  Run run = {-INFINITY, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
   // whole rounds of the block without a branch, the next one's loads under
   // way; then what is left
   constexpr int ROUND = NT * UNROLL;
@@ -254,22 +297,21 @@ __global__ void __launch_bounds__(NT)
 #pragma unroll
       for (int j = 0; j < N; ++j) x[u * N + j] = (float)v[u][j];
     if (r + 1 < rounds) load(r + 1);
-    take(x, UNROLL * N);
+    run.take(x);
   }
   for (int at = rounds * ROUND + tid; at < vecs; at += NT) {
     const V w = Vec<T>::load(part + (long)at * N);
     float x[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) x[j] = (float)w[j];
-    take(x, N);
+    run.take(x);
   }
   if (tid == NT - 1)
     for (int j = 0; j < tail; ++j) {
-      const float x = (float)part[(long)vecs * N + j];
-      take(&x, 1);
+      const float x[1] = {(float)part[(long)vecs * N + j]};
+      run.take(x);
     }
-  a.s += s1;
-  a.t += t1;
+  Stat a = run.stat();
 
   // the thread's maximum, and that of its group
   const bool any = tid < vecs || (tid == NT - 1 && tail > 0);
@@ -409,7 +451,9 @@ __global__ void __launch_bounds__(NT)
 #define SPLITS_MAX 64
 
 // Joins the splits of a row, one wave a row.  Lane l holds split l and its
-// sorted list, which waits in LDS; the largest head is taken k times.
+// sorted list.  If q is how many a list has to give on average, c lists
+// whose q-th elements are the largest hold k elements that reach the
+// smallest of those c: only what reaches that bar is ranked.
 template <typename T>
 __global__ void __launch_bounds__(WAVE)
     logprobs_join_kernel(const T* __restrict__ logits, long stride,
@@ -418,6 +462,10 @@ __global__ void __launch_bounds__(WAVE)
                          const unsigned long* __restrict__ pkeys, long C,
                          int splits, int k) {
   __shared__ unsigned long list[SPLITS_MAX * TOP_MAX];
+  __shared__ unsigned long cand[SPLITS_MAX * TOP_MAX];
+  __shared__ unsigned probes[WAVE];
+  __shared__ unsigned bar;
+  __shared__ int count;
   const long row = blockIdx.x;
   const int lane = threadIdx.x;
   const long token = token_of(tokens, row);
@@ -432,6 +480,10 @@ __global__ void __launch_bounds__(WAVE)
     const float* p = pstat + (row * splits + lane) * 3;
     a = {p[0], p[1], p[2]};
   }
+  if (lane == 0) {
+    bar = 0xFFFFFFFFu;
+    count = 0;
+  }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1)
     a = stat_join(a, {__shfl_xor(a.m, off, WAVE), __shfl_xor(a.s, off, WAVE),
@@ -439,18 +491,31 @@ __global__ void __launch_bounds__(WAVE)
   if (lane == 0) write_stats(out, row, a, logits + row * stride, C, token);
   if (k == 0) return;
   __syncthreads();
-  int at = 0;
-  unsigned long head = lane < splits ? list[lane * k] : 0;
-  unsigned long mine = 0;  // lane j keeps the j-th
-  for (int j = 0; j < k; ++j) {
-    const unsigned long top = wave_key_max(head);
-    if (lane == j) mine = top;
-    if (head == top && top != 0) {
-      ++at;
-      head = at < k ? list[lane * k + at] : 0;
+  const int q = (k + splits - 1) / splits, c = (k + q - 1) / q;
+  const unsigned mine =
+      lane < splits ? (unsigned)(list[lane * k + q - 1] >> 32) : 0;
+  probes[lane] = mine;
+  __syncthreads();
+  int above = 0;
+  for (int i = 0; i < splits; ++i) above += probes[i] > mine;
+  if (lane < splits && above < c) atomicMin(&bar, mine);
+  __syncthreads();
+  const unsigned least = max(bar, 1u);
+  if (lane < splits)
+    for (int j = 0; j < k; ++j) {
+      const unsigned long key = list[lane * k + j];
+      if ((unsigned)(key >> 32) < least) break;
+      cand[atomicAdd(&count, 1)] = key;
     }
+  __syncthreads();
+  const int n = count;
+  for (int i = lane; i < n; i += WAVE) {
+    const unsigned long key = cand[i];
+    int r = 0;
+    for (int j = 0; j < n; ++j) r += cand[j] > key ? 1 : 0;
+    if (r < k) write_top(out, row, k, r, key, a);
   }
-  if (lane < k) write_top(out, row, k, lane, mine, a);
+  for (int j = n + lane; j < k; j += WAVE) write_top(out, row, k, j, 0, a);
 }
 
 struct RowGrad {
