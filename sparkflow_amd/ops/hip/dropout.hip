@@ -51,7 +51,11 @@ __device__ __forceinline__ T drop(T x, unsigned w, unsigned last, float s) {
   return w <= last ? (T)y : (T)0.0f;
 }
 
-template <typename T, int UNROLL>
+// One vector of 16 bytes a thread: more of them (2: 47.6 us for 45.4, 4: 50.9
+// at 8192 x 8192 bf16) only lengthen a block.  That is 5.9 TB/s, 94% of what
+// a plain copy reaches; two Philox blocks for every eight elements of 16 bits
+// stay hidden behind it.
+template <typename T, bool LARGE>
 __global__ void __launch_bounds__(256)
     dropout_kernel(const T* __restrict__ x, T* __restrict__ y,
                    const long* __restrict__ state, long n, unsigned last,
@@ -59,37 +63,30 @@ __global__ void __launch_bounds__(256)
   constexpr int N = Vec<T>::N;
   const unsigned long seed = (unsigned long)state[0];
   const unsigned long offset = (unsigned long)state[1];
-  const long first =
-      ((long)blockIdx.x * (256 * UNROLL) + threadIdx.x) * N;
-  typename Vec<T>::V v[UNROLL];
+  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * N;
+  if (i + N <= n) {
+    typename Vec<T>::V v =
+        LARGE ? Vec<T>::load_once(x + i) : Vec<T>::load(x + i);
 #pragma unroll
-  for (int u = 0; u < UNROLL; ++u) {
-    const long i = first + (long)u * 256 * N;
-    if (i + N <= n) v[u] = Vec<T>::load(x + i);
-  }
+    for (int q = 0; q < N / 4; ++q) {
+      const Philox r = philox10((unsigned long)(i / 4 + q), offset, seed);
 #pragma unroll
-  for (int u = 0; u < UNROLL; ++u) {
-    const long i = first + (long)u * 256 * N;
-    if (i >= n) break;
-    if (i + N <= n) {
-#pragma unroll
-      for (int q = 0; q < N / 4; ++q) {
-        const Philox r = philox10((unsigned long)(i / 4 + q), offset, seed);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          v[u][4 * q + j] = drop(v[u][4 * q + j], r.w[j], last, scale);
-      }
-      Vec<T>::store(y + i, v[u]);
-    } else {
-      for (long e = i; e < n; ++e) {
-        const Philox r = philox10((unsigned long)(e / 4), offset, seed);
-        const unsigned w = e % 4 == 0   ? r.w[0]
-                           : e % 4 == 1 ? r.w[1]
-                           : e % 4 == 2 ? r.w[2]
-                                        : r.w[3];
-        y[e] = drop(x[e], w, last, scale);
-      }
+      for (int j = 0; j < 4; ++j)
+        v[4 * q + j] = drop(v[4 * q + j], r.w[j], last, scale);
     }
+    if (LARGE)
+      Vec<T>::store_once(y + i, v);
+    else
+      Vec<T>::store(y + i, v);
+    return;
+  }
+  for (long e = i; e < n; ++e) {
+    const Philox r = philox10((unsigned long)(e / 4), offset, seed);
+    const unsigned w = e % 4 == 0   ? r.w[0]
+                       : e % 4 == 1 ? r.w[1]
+                       : e % 4 == 2 ? r.w[2]
+                                    : r.w[3];
+    y[e] = drop(x[e], w, last, scale);
   }
 }
 
@@ -124,19 +121,20 @@ torch::Tensor dropout(torch::Tensor x, torch::Tensor state, int64_t keep,
   for_dtype(x.scalar_type(), "x", [&](auto t) {
     using T = decltype(t);
     const long vecs = (n + Vec<T>::N - 1) / Vec<T>::N;
-    auto go = [&](auto kernel, int unroll) {
-      const long blocks = (vecs + 256 * unroll - 1) / (256 * unroll);
+    auto go = [&](auto kernel) {
+      const long blocks = (vecs + 255) / 256;
       TORCH_CHECK(blocks < (1l << 31), "dropout: tensor too large");
       hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0,
                          stream, ptr<T>(x), ptr<T>(y),
                          state.data_ptr<int64_t>(), n,
                          (unsigned)(keep - 1), (float)scale);
     };
-    if (vecs >= 256l * 256 * 8) {
-      go(dropout_kernel<T, 2>, 2);
-    } else {
-      go(dropout_kernel<T, 1>, 1);
-    }
+    // Beyond the 256 MB of the last cache nothing of x or y would be found
+    // there again (8192 x 8192 bf16: 45.4 us for 47.5).
+    if (2 * n * (long)sizeof(T) >= 256l << 20)
+      go(dropout_kernel<T, true>);
+    else
+      go(dropout_kernel<T, false>);
   });
   LAUNCH_OK();
   return y;

@@ -55,17 +55,31 @@ __device__ __forceinline__ unsigned order_of(float x) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// A thread's own running sums, in steps of log 2 and about a whole number of
-// them: e^x / 2^shift is one exponential of one fused product, with one
-// rounding less than e^(x - m), and two instructions less an element, which
-// is what bounds the pass in the 16-bit types.  Two sums each, for shorter
-// chains.  Where m log2 e leaves fp32 (the lowest value as a mask of a whole
-// row) or is infinite, the sums are about m itself.
-struct Run {
-  float m, shift, s0, s1, t0, t1;
+// The join of all lanes, in every lane: one change of maximum, then sums.
+__device__ __forceinline__ Stat wave_join(Stat a) {
+  a = stat_at(a, wave_max(a.m));
+  return {a.m, wave_sum(a.s), wave_sum(a.t)};
+}
 
-  __device__ __forceinline__ bool far() const {
-    return !(fabsf(m) < 1.0e38f);
+// A thread's own running sums, in steps of log 2 and about a whole number of
+// them, `shift`: e^x / 2^shift is one exponential of one fused product, with
+// one rounding and two instructions less than e^(x - m), and instructions
+// are what bounds the pass in the 16-bit types.  The sums move to another
+// shift only when a value is 2.5 above `ref`, where they were put last: some
+// lane of a wave has a new maximum almost every time, and seldom one that
+// far.  Two sums each, for shorter chains.  Where ref log2 e leaves fp32 (the
+// lowest value as a mask of a whole row) or is infinite, the sums are about
+// ref itself.
+struct Run {
+  float m, ref, limit, shift, s0, s1, t0, t1;
+
+  __device__ __forceinline__ void clear() {
+    m = ref = limit = shift = -INFINITY;
+    s0 = s1 = t0 = t1 = 0.0f;
+  }
+
+  static __device__ __forceinline__ bool far(float ref) {
+    return !(fabsf(ref) < 1.0e38f);
   }
 
   // Adds n values.
@@ -75,28 +89,31 @@ struct Run {
     float gm = x[0];
 #pragma unroll
     for (int j = 1; j < n; ++j) gm = fmaxf(gm, x[j]);
-    if (gm > m) {  // seldom, but at the start
-      const Run old = *this;
-      m = gm;
+    m = fmaxf(m, gm);
+    if (gm > limit) {
+      const float old = ref, from = shift;
+      ref = gm;
       shift = rintf(gm * LOG2E);
-      if (old.m != -INFINITY) {
-        const float d = far() || old.far() ? (old.m - m) * LOG2E
-                                           : old.shift - shift;
+      limit = far(ref) ? ref : ref + 2.5f;
+      if (old != -INFINITY) {
+        const float d =
+            far(old) || far(ref) ? (old - ref) * LOG2E : from - shift;
         const float f = __builtin_amdgcn_exp2f(d);
-        // a maximum of infinite distance leaves nothing of the old sums
+        // a reference of infinite distance leaves nothing of the old sums
         const float g = fmaxf(d, -1000.0f);
-        s0 = old.s0 * f;
-        s1 = old.s1 * f;
-        t0 = (old.t0 + old.s0 * g) * f;
-        t1 = (old.t1 + old.s1 * g) * f;
+        t0 = (t0 + s0 * g) * f;
+        t1 = (t1 + s1 * g) * f;
+        s0 *= f;
+        s1 *= f;
       }
     }
-    if (far()) {
+    if (far(ref)) {
 #pragma unroll
       for (int j = 0; j < n; ++j) {
         // nothing but -inf so far: only a NaN says anything
-        const float d = m == -INFINITY ? (x[j] != x[j] ? x[j] : -INFINITY)
-                                       : (x[j] - m) * LOG2E;
+        const float d = ref == -INFINITY
+                            ? (x[j] != x[j] ? x[j] : -INFINITY)
+                            : (x[j] - ref) * LOG2E;
         const float e = __builtin_amdgcn_exp2f(d);
         s0 += e;
         t0 = fmaf(e, fmaxf(d, -1000.0f), t0);
@@ -123,7 +140,7 @@ struct Run {
   __device__ __forceinline__ Stat stat() const {
     constexpr float LOG2E = 1.44269504089f, LN2 = 0.69314718056f;
     const float s = s0 + s1, t = t0 + t1;
-    if (far()) return {m, s, t * LN2};
+    if (far(ref)) return {m, s, t * LN2};  // m is ref
     const float d = fmaf(m, LOG2E, -shift);
     const float f = __builtin_amdgcn_exp2f(-d);
     return {m, s * f, (t - s * d) * f * LN2};
@@ -209,18 +226,17 @@ __device__ __forceinline__ void write_ignored(const RowOut& o, long row,
   }
 }
 
-template <typename T>
+// x: the token's logit, NaN for a token that the row does not have.
 __device__ __forceinline__ void write_stats(const RowOut& o, long row,
-                                            Stat a, const T* xr, long C,
-                                            long token) {
+                                            Stat a, float x) {
   const float l = a.s == 0.0f ? 0.0f : logf(a.s);
   float lp;
-  if (token < 0 || token >= C) {
-    lp = NAN;  // no such token
+  if (x != x) {
+    lp = NAN;
   } else if (a.s == 0.0f) {
     lp = -INFINITY;  // every token of the row is impossible
   } else {
-    lp = ((float)xr[token] - a.m) - l;
+    lp = (x - a.m) - l;
   }
   o.logp[row] = lp;
   o.entropy[row] = a.s == 0.0f ? 0.0f : l - a.t / a.s;
@@ -271,6 +287,7 @@ __global__ void __launch_bounds__(NT)
     return;
   }
   const T* xr = logits + row * stride;
+  const float chosen = token >= 0 && token < C ? (float)xr[token] : NAN;
   const long lo = split * span;
   const long hi = lo + span < C ? lo + span : C;
   const T* part = xr + lo;
@@ -278,16 +295,28 @@ __global__ void __launch_bounds__(NT)
   const int tail = (int)((hi - lo) % N);
 
   // -- one pass
-  Run run = {-INFINITY, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-  // whole rounds of the block without a branch, the next one's loads under
-  // way; then what is left
+  Run run;
+  run.clear();
+  // rounds of the block, the next one's loads under way; only the last is
+  // cut, and filled up with what has no weight
   constexpr int ROUND = NT * UNROLL;
-  const int rounds = vecs / ROUND;
+  const int rounds = (vecs + ROUND - 1) / ROUND;
   V v[UNROLL];
   auto load = [&](int r) {
+    const int at = r * ROUND + tid;
+    if ((r + 1) * ROUND <= vecs) {
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
-      v[u] = Vec<T>::load(part + (long)(r * ROUND + u * NT + tid) * N);
+      for (int u = 0; u < UNROLL; ++u)
+        v[u] = Vec<T>::load(part + (long)(at + u * NT) * N);
+      return;
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[u][j] = (T)-INFINITY;
+      if (at + u * NT < vecs)
+        v[u] = Vec<T>::load(part + (long)(at + u * NT) * N);
+    }
   };
   if (rounds > 0) load(0);
   for (int r = 0; r < rounds; ++r) {
@@ -297,13 +326,6 @@ __global__ void __launch_bounds__(NT)
 #pragma unroll
       for (int j = 0; j < N; ++j) x[u * N + j] = (float)v[u][j];
     if (r + 1 < rounds) load(r + 1);
-    run.take(x);
-  }
-  for (int at = rounds * ROUND + tid; at < vecs; at += NT) {
-    const V w = Vec<T>::load(part + (long)at * N);
-    float x[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = (float)w[j];
     run.take(x);
   }
   if (tid == NT - 1)
@@ -330,10 +352,7 @@ __global__ void __launch_bounds__(NT)
   }
 
   // -- the block's (m, s, t)
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1)
-    a = stat_join(a, {__shfl_xor(a.m, off, WAVE), __shfl_xor(a.s, off, WAVE),
-                      __shfl_xor(a.t, off, WAVE)});
+  a = wave_join(a);
   if (lane == 0) wstat[wave] = a;
   __syncthreads();
   a = wstat[0];
@@ -341,7 +360,7 @@ __global__ void __launch_bounds__(NT)
   for (int w = 1; w < NT / WAVE; ++w) a = stat_join(a, wstat[w]);
   if (tid == 0) {
     if (splits == 1) {
-      write_stats(out, row, a, xr, C, token);
+      write_stats(out, row, a, chosen);
     } else {
       float* p = pstat + ((long)row * splits + split) * 3;
       p[0] = a.m;
@@ -407,6 +426,7 @@ __global__ void __launch_bounds__(NT)
     for (int i = tid; i < n; i += NT) {
       const unsigned long key = cand[i];
       int r = 0;
+#pragma unroll 8
       for (int j = 0; j < n; ++j) r += cand[j] > key ? 1 : 0;
       if (r < k) emit(r, key);
     }
@@ -463,18 +483,23 @@ __global__ void __launch_bounds__(WAVE)
                          int splits, int k) {
   __shared__ unsigned long list[SPLITS_MAX * TOP_MAX];
   __shared__ unsigned long cand[SPLITS_MAX * TOP_MAX];
-  __shared__ unsigned probes[WAVE];
+  __shared__ __attribute__((aligned(16))) unsigned probes[WAVE];
   __shared__ unsigned bar;
   __shared__ int count;
   const long row = blockIdx.x;
   const int lane = threadIdx.x;
   const long token = token_of(tokens, row);
-  if (token == tokens.ignore) {
-    write_ignored(out, row, k, lane, WAVE);
-    return;
+  // (what an ignored row's splits left unwritten is loaded and not used)
+  const unsigned long* from = pkeys + row * splits * k;
+  for (int i0 = lane; i0 < splits * k; i0 += 8 * WAVE) {
+    unsigned long some[8];  // eight loads under way
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      some[u] = i0 + u * WAVE < splits * k ? from[i0 + u * WAVE] : 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (i0 + u * WAVE < splits * k) list[i0 + u * WAVE] = some[u];
   }
-  for (int i = lane; i < splits * k; i += WAVE)
-    list[i] = pkeys[row * splits * k + i];
   Stat a = {-INFINITY, 0.0f, 0.0f};
   if (lane < splits) {
     const float* p = pstat + (row * splits + lane) * 3;
@@ -484,20 +509,27 @@ __global__ void __launch_bounds__(WAVE)
     bar = 0xFFFFFFFFu;
     count = 0;
   }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1)
-    a = stat_join(a, {__shfl_xor(a.m, off, WAVE), __shfl_xor(a.s, off, WAVE),
-                      __shfl_xor(a.t, off, WAVE)});
-  if (lane == 0) write_stats(out, row, a, logits + row * stride, C, token);
+  if (token == tokens.ignore) {
+    write_ignored(out, row, k, lane, WAVE);
+    return;
+  }
+  const float chosen =
+      token >= 0 && token < C ? (float)logits[row * stride + token] : NAN;
+  a = wave_join(a);
+  if (lane == 0) write_stats(out, row, a, chosen);
   if (k == 0) return;
   __syncthreads();
   const int q = (k + splits - 1) / splits, c = (k + q - 1) / q;
   const unsigned mine =
       lane < splits ? (unsigned)(list[lane * k + q - 1] >> 32) : 0;
-  probes[lane] = mine;
+  probes[lane] = mine;  // 0 behind the last split: above no one
   __syncthreads();
   int above = 0;
-  for (int i = 0; i < splits; ++i) above += probes[i] > mine;
+#pragma unroll
+  for (int i = 0; i < WAVE; i += 4) {
+    const uint4 g = *reinterpret_cast<const uint4*>(&probes[i]);
+    above += (g.x > mine) + (g.y > mine) + (g.z > mine) + (g.w > mine);
+  }
   if (lane < splits && above < c) atomicMin(&bar, mine);
   __syncthreads();
   const unsigned least = max(bar, 1u);
@@ -512,6 +544,7 @@ __global__ void __launch_bounds__(WAVE)
   for (int i = lane; i < n; i += WAVE) {
     const unsigned long key = cand[i];
     int r = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) r += cand[j] > key ? 1 : 0;
     if (r < k) write_top(out, row, k, r, key, a);
   }

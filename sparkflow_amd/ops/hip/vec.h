@@ -25,6 +25,15 @@ struct Vec {
   static __device__ __forceinline__ void store(T* p, V v) {
     reinterpret_cast<Unaligned*>(p)->v = v;
   }
+  // For what is read or written once and is larger than the caches: it does
+  // not displace what they hold.
+  static __device__ __forceinline__ V load_once(const T* p) {
+    return __builtin_nontemporal_load(
+        &reinterpret_cast<const Unaligned*>(p)->v);
+  }
+  static __device__ __forceinline__ void store_once(T* p, V v) {
+    __builtin_nontemporal_store(v, &reinterpret_cast<Unaligned*>(p)->v);
+  }
 };
 
 // Calls f(T()) with the kernel's type for a tensor's dtype.
