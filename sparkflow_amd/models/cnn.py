@@ -50,6 +50,11 @@ class MNISTCNN(nn.Module):
     def predict(self, x):
         return F.argmax_rows(self.forward(x))
 
+    @torch.no_grad()
+    def score(self, x, labels, top_k: int = 0):
+        """As ClassifierMLP.score."""
+        return F.token_logprobs(self.forward(x), labels, top_k)
+
 
 class _BasicBlock(nn.Module):
     def __init__(self, cin, cout, stride, layout="nhwc"):
@@ -126,3 +131,8 @@ class ResNet18Shape(nn.Module):
     @torch.no_grad()
     def predict(self, x):
         return F.argmax_rows(self.forward(x))
+
+    @torch.no_grad()
+    def score(self, x, labels, top_k: int = 0):
+        """As ClassifierMLP.score."""
+        return F.token_logprobs(self.forward(x), labels, top_k)

@@ -36,6 +36,12 @@ class ClassifierMLP(nn.Module):
     def predict(self, x):
         return F.argmax_rows(self.forward(x))
 
+    @torch.no_grad()
+    def score(self, x, labels, top_k: int = 0):
+        """Log-probability of each row's label, the entropy of its
+        prediction and its ``top_k`` best classes (F.token_logprobs)."""
+        return F.token_logprobs(self.forward(x), labels, top_k)
+
 
 class RegressorMLP(nn.Module):
     """Dense stack with a sigmoid scalar head + MSE loss (reference
@@ -64,16 +70,17 @@ class DropoutRegressorMLP(nn.Module):
     """RegressorMLP with an inter-layer Dropout — exercises the
     reference's tf_dropout / to_keep_dropout surface (ml_util.py:70-71):
     dropout is active in training and inert at prediction for both
-    flag values."""
+    flag values.  With a ``seed`` its masks come from a counter
+    (snn.Dropout)."""
 
-    def __init__(self, dims: List[int], p: float = 0.3):
+    def __init__(self, dims: List[int], p: float = 0.3, seed: int = None):
         super().__init__()
         layers = []
         for i in range(len(dims) - 1):
             act = "relu" if i < len(dims) - 2 else "sigmoid"
             layers.append(snn.Linear(dims[i], dims[i + 1], activation=act))
         self.layers = nn.ModuleList(layers)
-        self.drop = snn.Dropout(p)
+        self.drop = snn.Dropout(p, seed=seed)
         self.loss_fn = snn.MSE()
 
     def forward(self, x):

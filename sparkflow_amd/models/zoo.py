@@ -55,7 +55,8 @@ def gaussian_mlp(in_dim: int = 10, hidden: int = 256):
     return RegressorMLP([in_dim, hidden, 1])
 
 
-def dropout_mlp(in_dim: int = 10, hidden: int = 64, p: float = 0.3):
+def dropout_mlp(in_dim: int = 10, hidden: int = 64, p: float = 0.3,
+                seed: int = None):
     """gaussian_mlp + inter-layer Dropout (the reference's tf_dropout
     surface, ml_util.py:70-71)."""
-    return DropoutRegressorMLP([in_dim, hidden, 1], p=p)
+    return DropoutRegressorMLP([in_dim, hidden, 1], p=p, seed=seed)

@@ -143,18 +143,93 @@ class BatchNorm2d(nn.Module):
 
 class Dropout(nn.Module):
     """Inverted dropout; inert in eval mode (the inference path — parity
-    with the reference's keep-prob feed at prediction, ml_util.py:70-71)."""
+    with the reference's keep-prob feed at prediction, ml_util.py:70-71).
 
-    def __init__(self, p: float = 0.5):
+    With a ``seed`` the masks come from a counter-based generator and are
+    not stored for backward (F.dropout): each forward draws the next one,
+    also at every replay of a captured step.  The seed belongs to the
+    builder, so every worker of a job draws the same sequence from it;
+    ``reseed`` starts another.  Without one, torch's generator and a stored
+    mask are used.
+    """
+
+    def __init__(self, p: float = 0.5, seed: int = None):
         super().__init__()
         self.p = p
+        # not part of the state dict: artifacts stay loadable either way
+        self.register_buffer(
+            "rng_state", None if seed is None else F.dropout_state(seed),
+            persistent=False)
+
+    def reseed(self, seed: int, offset: int = 0) -> None:
+        if getattr(self, "rng_state", None) is None:
+            raise ValueError("this Dropout was built without a seed")
+        # in place: a captured step keeps reading this tensor
+        self.rng_state.copy_(F.dropout_state(seed, offset))
 
     def forward(self, x):
         if not self.training or self.p <= 0:
             return x
+        state = getattr(self, "rng_state", None)  # None in older artifacts
+        if state is not None:
+            return F.dropout(x, self.p, F.dropout_next(state))
         keep = 1.0 - self.p
         mask = (torch.rand_like(x) < keep).to(x.dtype) / keep
         return x * mask
+
+
+class AdapterLinear(nn.Module):
+    """A frozen Linear with low-rank adapters beside it:
+    act(x W + bias + scale (x A_e^T) B_e^T), e the adapter of the row.
+
+    Only the adapters train, so only they are packed, pushed and pulled: at
+    rank r a layer sends r (in + out) numbers an adapter and not in * out.
+    ``forward(x, ids)`` takes one adapter a row (negative: none) or the
+    F.adapter_groups of them; without ids every row goes through adapter 0.
+    B starts at zero, so a new layer answers as its Linear does.
+    """
+
+    def __init__(self, in_features: int, out_features: int, rank: int,
+                 adapters: int = 1, scale: float = 1.0,
+                 activation: str = "none", bias: bool = True):
+        super().__init__()
+        self.in_features, self.out_features = in_features, out_features
+        self.rank, self.adapters, self.scale = rank, adapters, float(scale)
+        self.activation = activation
+        self.weight = nn.Parameter(
+            _glorot((in_features, out_features), in_features, out_features),
+            requires_grad=False)
+        self.bias = nn.Parameter(torch.zeros(out_features),
+                                 requires_grad=False) if bias else None
+        self.a = nn.Parameter(
+            _glorot((adapters, rank, in_features), in_features, rank))
+        self.b = nn.Parameter(torch.zeros(adapters, out_features, rank))
+
+    @classmethod
+    def from_linear(cls, linear: Linear, rank: int, adapters: int = 1,
+                    scale: float = 1.0) -> "AdapterLinear":
+        """Adapters beside a trained layer, whose weights are copied."""
+        layer = cls(linear.in_features, linear.out_features, rank, adapters,
+                    scale, linear.activation, linear.bias is not None)
+        layer.to(linear.weight.device)
+        with torch.no_grad():
+            layer.weight.copy_(linear.weight)
+            if linear.bias is not None:
+                layer.bias.copy_(linear.bias)
+        return layer
+
+    def forward(self, x, ids=None):
+        if ids is None:
+            ids = torch.zeros(x.shape[:-1], dtype=torch.int64,
+                              device=x.device)
+        base = F.linear_act(x, self.weight, self.bias, "none")
+        return F.adapter_add(base, x, self.a, self.b, ids, self.scale,
+                             self.activation)
+
+    def extra_repr(self):
+        return (f"{self.in_features}->{self.out_features}, "
+                f"adapters={self.adapters} of rank {self.rank}, "
+                f"act={self.activation}")
 
 
 class SoftmaxCrossEntropy(nn.Module):

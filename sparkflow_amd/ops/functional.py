@@ -123,6 +123,16 @@ class LinearAct(torch.autograd.Function):
         act = ctx.act
         need_dx = ctx.needs_input_grad[0]
         dy = dy.contiguous()
+        if not (ctx.needs_input_grad[1] or ctx.needs_input_grad[2]):
+            # a frozen layer (adapters train beside it): no weight grads
+            if not need_dx:
+                return None, None, None, None
+            if ops.use_hip(x):
+                dx = ops.hip.gemm_dgrad_act(dy, y, w, act) \
+                    if act != ACT_NONE else ops.hip.gemm_dgrad(dy, w)
+            else:
+                dx = _act_bwd_from_out(y, dy, act) @ w.t()
+            return dx, None, None, None
         if ops.use_hip(x):
             import os
 

@@ -289,3 +289,195 @@ def test_adapter_add_refuses():
             F.adapter_groups(ids, e)
     with pytest.raises(KeyError):
         F.adapter_add(base, x, a, b, ids, act="tanh")
+
+
+# -- modules and models -------------------------------------------------------
+
+
+def test_dropout_module_with_a_seed():
+    from sparkflow_amd import nn as snn
+
+    old, new = snn.Dropout(0.4), snn.Dropout(0.4, seed=7)
+    assert list(new.state_dict()) == []  # artifacts of either load as both
+    x = torch.ones(4, 50)
+    assert torch.equal(new(x), F.dropout(x, 0.4, F.dropout_state(7, 0)))
+    assert torch.equal(new(x), F.dropout(x, 0.4, F.dropout_state(7, 1)))
+    new.reseed(9, 3)
+    assert torch.equal(new(x), F.dropout(x, 0.4, F.dropout_state(9, 3)))
+    assert new.eval()(x) is x
+    # without a seed: torch's generator, as before
+    torch.manual_seed(3)
+    want = x * ((torch.rand_like(x) < 0.6).to(x.dtype) / 0.6)
+    torch.manual_seed(3)
+    assert torch.equal(old(x), want)
+    with pytest.raises(ValueError, match="without a seed"):
+        old.reseed(1)
+
+
+def _seeded_dropout_mlp():
+    from sparkflow_amd.models import dropout_mlp
+
+    return dropout_mlp(in_dim=6, hidden=16, p=0.3, seed=5)
+
+
+def test_seeded_dropout_model_serializes():
+    from sparkflow_amd.graph_utils import build_graph
+    from sparkflow_amd.models import dropout_mlp
+    from sparkflow_amd.utils.serialization import module_from_json
+
+    again = module_from_json(build_graph(_seeded_dropout_mlp))
+    assert again.drop.rng_state.tolist() == [5, 0]
+    plain = dropout_mlp(in_dim=6, hidden=16)
+    assert list(plain.state_dict()) == list(again.state_dict())
+    x, y = torch.randn(8, 6), torch.rand(8, 1)
+    again.train().compute_loss(again(x), y).backward()
+    assert all(torch.isfinite(p.grad).all() for p in again.parameters())
+
+
+def test_adapter_linear_module():
+    from sparkflow_amd import nn as snn
+    from sparkflow_amd.utils.serialization import flat_size, param_list
+
+    linear = snn.Linear(12, 7, activation="relu")
+    layer = snn.AdapterLinear.from_linear(linear, rank=3, adapters=4,
+                                          scale=0.5)
+    x = torch.randn(10, 12)
+    assert torch.equal(layer(x), linear(x))  # B is zero at first
+    assert [id(p) for p in param_list(layer)] == [id(layer.a), id(layer.b)]
+    assert flat_size(layer) == 4 * 3 * (12 + 7)
+    with torch.no_grad():
+        layer.b.normal_()
+    ids = torch.tensor([0, 1, 2, 3, -1, 3, 2, 1, 0, -1])
+    base = F.linear_act(x, linear.weight, linear.bias)
+    value, tol = oracle.adapter(base.detach(), x, layer.a, layer.b, ids,
+                                0.5)[0]
+    got = layer(x, ids)
+    assert ((got.double() - torch.relu(value)).abs() <= tol).all()
+    assert torch.equal(layer(x, F.adapter_groups(ids, 4)), got)
+    x.requires_grad_()
+    layer(x, ids).sum().backward()
+    assert layer.weight.grad is None and layer.bias.grad is None
+    assert layer.a.grad is not None and x.grad is not None
+
+
+def test_frozen_linear_gradient_of_x():
+    for act in ("none", "relu", "sigmoid"):
+        x, w, b = torch.randn(5, 6), torch.randn(6, 4), torch.randn(4)
+        one = x.clone().requires_grad_()
+        F.linear_act(one, w, b, act).sum().backward()
+        two, w2 = x.clone().requires_grad_(), w.clone().requires_grad_()
+        F.linear_act(two, w2, b, act).sum().backward()
+        torch.testing.assert_close(one.grad, two.grad)
+
+
+def test_classifier_score():
+    from sparkflow_amd.models import mnist_mlp
+
+    model = mnist_mlp()
+    x, labels = torch.randn(5, 784), torch.tensor([3, 1, 4, 1, 5])
+    r = model.score(x, labels.float().unsqueeze(1), top_k=2)
+    logp = torch.log_softmax(model(x), 1)
+    torch.testing.assert_close(r.logp, logp[torch.arange(5), labels])
+    assert torch.equal(r.top_ids[:, 0].float(), model.predict(x))
+
+
+class _AdaptedClassifier(torch.nn.Module):
+    """Fine-tuning as a user writes it: dropout on the input of adapters
+    beside frozen layers, against the log-probabilities of the answers and
+    a reward for entropy."""
+
+    def __init__(self, dims, rank, adapters, seed):
+        super().__init__()
+        from sparkflow_amd import nn as snn
+
+        self.drop = snn.Dropout(0.2, seed=seed)
+        self.hidden = snn.AdapterLinear(dims[0], dims[1], rank, adapters,
+                                        activation="relu")
+        self.out = snn.AdapterLinear(dims[1], dims[2], rank, adapters)
+
+    def forward(self, x, ids=None):
+        return self.out(self.hidden(self.drop(x), ids), ids)
+
+    def compute_loss(self, out, target):
+        r = F.token_logprobs(out, target)
+        return -(r.logp + 0.01 * r.entropy).mean()
+
+
+def check_operators_together(device, rows=20):
+    """Dropout, adapters and log-probabilities in one training step, against
+    autograd over plain operations in 64 bits."""
+    torch.manual_seed(0)
+    model = _AdaptedClassifier([12, 9, 6], 2, 3, seed=11)
+    with torch.no_grad():
+        for p in (model.hidden.b, model.out.b):
+            p.normal_(std=0.3)
+    x, ids = torch.randn(rows, 12), torch.randint(-1, 3, (rows,))
+    y = torch.randint(0, 6, (rows,))
+    y[4] = -100
+    model.to(device)
+    loss = model.compute_loss(
+        model(x.to(device), F.adapter_groups(ids.to(device), 3)),
+        y.to(device))
+    loss.backward()
+
+    keep = oracle.kept(F.dropout_state(11), 0.2, x.numel()).reshape(x.shape)
+    leaves = {n: p.detach().cpu().double().requires_grad_()
+              for n, p in model.named_parameters()}
+    h = x.double() * keep / 0.8
+    mine = (ids.unsqueeze(1) == torch.arange(3)).double()
+    for layer in ("hidden", "out"):
+        w, bias, a, b = (leaves["%s.%s" % (layer, n)]
+                         for n in ("weight", "bias", "a", "b"))
+        z = torch.einsum("mk,erk->mer", h, a) * mine.unsqueeze(2)
+        h = h @ w + bias + torch.einsum("mer,enr->mn", z, b)
+        if layer == "hidden":
+            h = torch.relu(h)
+    logp = torch.log_softmax(h, 1)
+    live = y != -100
+    chosen = logp[torch.arange(rows), y.clamp(min=0)] * live
+    entropy = -(logp.exp() * logp).sum(1) * live
+    want = -(chosen + 0.01 * entropy).mean()
+    want.backward()
+    torch.testing.assert_close(loss.cpu().double(), want, rtol=1e-5,
+                               atol=1e-6)
+    for n, p in model.named_parameters():
+        if p.requires_grad:
+            torch.testing.assert_close(p.grad.cpu().double(),
+                                       leaves[n].grad, rtol=1e-4, atol=1e-6)
+
+
+def test_operators_together():
+    check_operators_together("cpu")
+
+
+def _adapted_builder():
+    from tests.test_lm_ops_cpu import _AdaptedClassifier
+
+    torch.manual_seed(1)
+    return _AdaptedClassifier([10, 16, 4], 2, 1, seed=3)
+
+
+def test_adapters_train_through_the_engine():
+    import numpy as np
+
+    from sparkflow_amd.graph_utils import build_graph
+    from sparkflow_amd.parallel.ps import OptimizerSpec, PSCore, TrainConfig
+    from sparkflow_amd.parallel.transport import LocalTransport
+    from sparkflow_amd.parallel.worker import Worker
+
+    graph_json = build_graph(_adapted_builder)
+    ps = PSCore(graph_json, OptimizerSpec("adam", 0.01), device="cpu")
+    before = ps.weights.clone()
+    assert before.numel() == 2 * (10 + 16) + 2 * (16 + 4)
+    worker = Worker(graph_json, LocalTransport(ps, "cpu"),
+                    TrainConfig(iters=3, mini_batch=8,
+                                mini_stochastic_iters=1, seed=0),
+                    device="cpu")
+    frozen = worker.module.hidden.weight.clone()
+    rng = np.random.default_rng(0)
+    worker.run(rng.random((24, 10), dtype=np.float32),
+               rng.integers(0, 4, (24, 1)).astype(np.float32))
+    assert ps.update_count == 3
+    assert torch.isfinite(ps.weights).all()
+    assert not torch.equal(ps.weights, before)
+    assert torch.equal(worker.module.hidden.weight, frozen)

@@ -679,3 +679,100 @@ def test_adapter_captured_and_streams():
         torch.cuda.synchronize()
         for p, q in zip(held, step()):
             assert torch.equal(p, q)
+
+
+# -- modules and the engine ---------------------------------------------------
+
+
+@pytest.mark.parametrize("rows", [20, 90, 1500])
+def test_operators_together_gpu(rows):
+    from tests.test_lm_ops_cpu import check_operators_together
+
+    check_operators_together(DEV, rows)
+
+
+def test_no_second_derivative():
+    """An error, not a silent zero."""
+    x = _randn(4, 9).requires_grad_()
+    r = F.token_logprobs(x, torch.zeros(4, device=DEV))
+    (g,) = torch.autograd.grad(r.logp.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="only once"):
+        g.sum().backward()
+    base, x, a, b, ids, scale = _adapter_inputs(9, 8, 7, 2, 2)
+    a.requires_grad_()
+    y = F.adapter_add(base, x, a, b, ids, scale=scale)
+    (g,) = torch.autograd.grad(y.sum(), a, create_graph=True)
+    with pytest.raises(RuntimeError, match="only once"):
+        g.sum().backward()
+
+
+def test_changed_inputs_are_noticed():
+    """What backward needs may not change before it runs."""
+    state = F.dropout_state(1, device=DEV)
+    x = _randn(8).requires_grad_()
+    y = F.dropout(x, 0.5, state)
+    state.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+    base, x, a, b, ids, scale = _adapter_inputs(9, 8, 7, 2, 2)
+    a.requires_grad_()
+    y = F.adapter_add(base, x, a, b, ids, scale=scale)
+    ids.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+    groups = F.adapter_groups(ids, 2)  # keeps its own copy
+    want = F.adapter_add(base, x, a, b, groups, scale=scale)
+    ids.fill_(1)
+    assert torch.equal(F.adapter_add(base, x, a, b, groups, scale=scale),
+                       want)
+
+
+@pytest.mark.parametrize("model", ["dropout", "adapters"])
+def test_captured_training_steps(model):
+    """The engine's captured step: a new mask at each replay, and weights
+    that move."""
+    from sparkflow_amd.graph_utils import build_graph
+    from sparkflow_amd.parallel.ps import OptimizerSpec, PSCore, TrainConfig
+    from sparkflow_amd.parallel.transport import LocalTransport
+    from sparkflow_amd.parallel.worker import Worker
+    from tests.test_lm_ops_cpu import _adapted_builder, _seeded_dropout_mlp
+
+    width, build = {"dropout": (6, _seeded_dropout_mlp),
+                    "adapters": (10, _adapted_builder)}[model]
+    graph_json = build_graph(build)
+    ps = PSCore(graph_json, OptimizerSpec("adam", 0.01), device=DEV)
+    worker = Worker(graph_json, LocalTransport(ps, DEV),
+                    TrainConfig(iters=1, seed=0), device=DEV)
+    rng = np.random.default_rng(0)
+    y = rng.integers(0, 2, (64, 1)).astype(np.float32)
+    worker.stage(rng.random((64, width), dtype=np.float32), y)
+    worker.run_steps(4, 16, use_graph=True)
+    torch.cuda.synchronize()
+    drawn = int(worker.module.drop.rng_state[1])
+    before = ps.weights.clone()
+    seen = []
+    for _ in range(3):
+        worker.run_steps(2, 16, use_graph=True)
+        torch.cuda.synchronize()
+        seen.append(ps.weights.clone())
+        with torch.no_grad():  # the program's own work between replays
+            worker.module(worker.x).sum().item()
+    # an eager forward in between draws as well
+    assert int(worker.module.drop.rng_state[1]) == drawn + 3 * 3
+    for weights in seen:
+        assert torch.isfinite(weights).all()
+        assert not torch.equal(weights, before)
+        before = weights
+
+
+def test_mnist_cnn_score_gpu():
+    from sparkflow_amd.models import mnist_cnn
+
+    model = mnist_cnn().to(DEV)
+    x = _randn(6, 784)
+    labels = torch.arange(6, device=DEV).float().unsqueeze(1)
+    r = model.score(x, labels, top_k=3)
+    logp, h, top, ids = oracle.logprobs(model(x), labels.squeeze(1), 3)
+    assert torch.equal(r.top_ids.cpu(), ids)
+    _within(r.logp, logp, oracle.logprobs_tol(logp, False, 10))
+    assert torch.equal(r.top_ids[:, 0].float(), model.predict(x))
