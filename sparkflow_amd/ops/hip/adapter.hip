@@ -282,7 +282,9 @@ __device__ __forceinline__ Split split(const float (&x)[8]) {
 
 // z[place][r] = s_e sum_k x[row][k] W_e(r, k).  W is [R, K] (KMAJOR) or
 // [K, R].  One block takes SUB tiles of an adapter, which share its loads of
-// W; its waves take turns along k and meet in LDS.
+// W; its waves take turns along k and meet in LDS.  A few rows may be split
+// over blocks along k too (gridDim.y): each writes a plane of z of its own,
+// and expand adds them up.
 template <typename T, int RB, bool KMAJOR, bool SMALL, int WAVES, int SUB,
           int U>
 __global__ void __launch_bounds__(WAVES * WAVE)
@@ -336,7 +338,8 @@ __global__ void __launch_bounds__(WAVES * WAVE)
   // as a rule, and blocks that walk them in step meet in a few channels of
   // the memory.
   const int turn = whole > 0 ? (int)blockIdx.x * WAVES % whole : 0;
-  for (int c0 = wave; c0 < whole; c0 += WAVES) {
+  const int from = wave + WAVES * blockIdx.y, stride = WAVES * gridDim.y;
+  for (int c0 = from; c0 < whole; c0 += stride) {
     const int c = c0 + turn < whole ? c0 + turn : c0 + turn - whole;
     V xv[U][SUB], wv[U][RB];
 #pragma unroll
@@ -355,8 +358,8 @@ __global__ void __launch_bounds__(WAVES * WAVE)
         for (int rb = 0; rb < RB; ++rb)
           acc[s][rb] = mma(xv[u][s], wv[u][rb], acc[s][rb]);
   }
-  for (int k0 = whole * (STEP * U) + wave * STEP; k0 < K;
-       k0 += WAVES * STEP) {
+  for (int k0 = whole * (STEP * U) + from * STEP; k0 < K;
+       k0 += stride * STEP) {
     const int k = k0 + quarter * N;
     V xv[SUB], wv[RB];
     if (k + N <= K) {
@@ -392,6 +395,7 @@ __global__ void __launch_bounds__(WAVES * WAVE)
       part[wave][s * RB + rb][lane] = acc[s][rb];
   __syncthreads();
   const float f = scales ? scales[t[0].g] : scale;
+  float* plane = z + (long)blockIdx.y * p.M * (RB * 16);
   // whole waves: a wave's 64 lanes finish the 16 x 16 of one (s, rb)
   for (int b = wave; b < SUB * RB; b += WAVES) {
     f32x4 sum = part[0][b][lane];
@@ -406,7 +410,7 @@ __global__ void __launch_bounds__(WAVES * WAVE)
         const int m = quarter * 4 + q;
         const long place = __shfl(t[s].place, m, WAVE);
         if (m < t[s].rows)
-          z[place * (RB * 16) + r] = r < R ? f * sum[q] : 0.0f;
+          plane[place * (RB * 16) + r] = r < R ? f * sum[q] : 0.0f;
       }
     }
   }
@@ -435,7 +439,7 @@ __global__ void __launch_bounds__(WAVES * WAVE)
                           const float* __restrict__ z,
                           const T* __restrict__ w, Plan p,
                           T* __restrict__ out, int N, int R, int act,
-                          int across) {
+                          int across, int planes) {
   constexpr int V = Vec<T>::N;
   constexpr int COLS = 16 * V;
   constexpr int THREADS = WAVES * WAVE;
@@ -563,15 +567,24 @@ __global__ void __launch_bounds__(WAVES * WAVE)
   // fills only half of the 32 that a bf16 instruction sums over: there the
   // high parts take one half and the middle parts the other.
   constexpr int ZB = BF16 ? 1 : RB, ZP = BF16 ? (RB + 1) / 2 : 1;
+  const float* zr = z + (long)t.place * (RB * 16);
+  auto load_z = [&](int r) {
+    f32x4 sum = *reinterpret_cast<const f32x4*>(zr + r);
+    if (SMALL) {
+#pragma unroll 4
+      for (int s = 1; s < planes; ++s)
+        sum += *reinterpret_cast<const f32x4*>(
+            zr + (long)s * p.M * (RB * 16) + r);
+    }
+    return sum;
+  };
   f32x4 zv[ZB];
   Vec<bf16_t>::V zh[ZP], zm[ZP], zl[ZP];
   if (adapted && BF16) {
 #pragma unroll
     for (int b = 0; b < ZP; ++b) {
       const int r = 32 * b + 8 * (RB == 1 ? quarter & 1 : quarter);
-      const float* from = z + (long)t.place * (RB * 16) + r;
-      const f32x4 lo = *reinterpret_cast<const f32x4*>(from);
-      const f32x4 hi = *reinterpret_cast<const f32x4*>(from + 4);
+      const f32x4 lo = load_z(r), hi = load_z(r + 4);
       const float f[8] = {lo[0], lo[1], lo[2], lo[3],
                           hi[0], hi[1], hi[2], hi[3]};
       const Split s = split(f);
@@ -588,9 +601,7 @@ __global__ void __launch_bounds__(WAVES * WAVE)
     }
   } else if (adapted) {
 #pragma unroll
-    for (int c = 0; c < ZB; ++c)
-      zv[c] = *reinterpret_cast<const f32x4*>(
-          z + (long)t.place * (RB * 16) + 16 * c + 4 * quarter);
+    for (int c = 0; c < ZB; ++c) zv[c] = load_z(16 * c + 4 * quarter);
   }
   for (int turn = 0; n0 < N; n0 += step, ++turn) {
     T* const part = wl[turn % BUFFERS];
@@ -711,18 +722,29 @@ __device__ __forceinline__ int first_slot(const Plan& p, int e,
 // elements j are one operand, beside z in three parts.  KMAJOR: the result is [R, K] (dA), else [K, R]
 // (dB).  SMALL_OUTER, DIRECT_OUTER: one block an adapter, rounded into out;
 // SPLIT_OUTER: one block a stretch, into fp32 sums that reduce joins.
+// One of the two: dA from x and dz, or dB from dy and z.
+template <typename T>
+struct OuterSide {
+  const T* x;
+  long xstride;
+  const float* z;
+  T* out;
+  float* partial;
+  int K, chunks, stretch;  // chunks of 16 V columns; 0: not wanted
+};
+
 template <typename T, int RB, bool KMAJOR, OuterWork WORK>
-__global__ void __launch_bounds__(256)
-    adapter_outer_kernel(const T* __restrict__ x, long xstride,
-                         const float* __restrict__ z, int zstride, Plan p,
-                         T* __restrict__ out, float* __restrict__ partial,
-                         int K, int R, int stretch) {
+__device__ __forceinline__ void outer_block(
+    const OuterSide<T>& side, const Plan& p, int zstride, int R, int column,
+    f32x4 (&part)[2][RB * Vec<T>::N][WAVE], int (&list)[SMALL_ROWS],
+    int& found) {
   constexpr int V = Vec<T>::N;
   constexpr bool BF16 = std::is_same<T, bf16_t>::value;
   constexpr int U = BF16 ? 8 : 4;
-  __shared__ f32x4 part[2][RB * V][WAVE];
-  __shared__ int list[SMALL_ROWS];
-  __shared__ int found;
+  const T* __restrict__ x = side.x;
+  const float* __restrict__ z = side.z;
+  const long xstride = side.xstride;
+  const int K = side.K, stretch = side.stretch;
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
   const int i = lane & 15, quarter = lane >> 4;
   int begin = 0, end = 0;
@@ -752,7 +774,7 @@ __global__ void __launch_bounds__(256)
     end = min(p.seg[found + 1], begin + stretch * TILE);
   }
   const int r0 = blockIdx.z * (RB * 16);
-  const int k0 = blockIdx.x * (16 * V);
+  const int k0 = column * (16 * V);
   const int k = k0 + i * V;
   f32x4 acc[RB][V] = {};
   // The bf16 loop: 32 rows a step.  Nothing but the rows' numbers is loaded
@@ -932,13 +954,13 @@ __global__ void __launch_bounds__(256)
       for (int q = 0; KMAJOR && q < 4; ++q)
 #pragma unroll
         for (int h = 0; h < V / 4; ++h)
-          Vec<float>::store(partial + o0 + (long)(r + q) * K + k + 4 * h,
+          Vec<float>::store(side.partial + o0 + (long)(r + q) * K + k + 4 * h,
                             f32x4{acc[c][4 * h][q], acc[c][4 * h + 1][q],
                                   acc[c][4 * h + 2][q],
                                   acc[c][4 * h + 3][q]});
 #pragma unroll
       for (int j = 0; !KMAJOR && j < V; ++j)
-        Vec<float>::store(partial + o0 + (long)(k + j) * R + r, acc[c][j]);
+        Vec<float>::store(side.partial + o0 + (long)(k + j) * R + r, acc[c][j]);
       continue;
     }
 #pragma unroll
@@ -949,28 +971,46 @@ __global__ void __launch_bounds__(256)
         const long o = o0 + (KMAJOR ? (long)(r + q) * K + k + j
                                     : (long)(k + j) * R + r + q);
         if (WORK == SPLIT_OUTER)
-          partial[o] = acc[c][j][q];
+          side.partial[o] = acc[c][j][q];
         else
-          out[o] = (T)acc[c][j][q];
+          side.out[o] = (T)acc[c][j][q];
       }
   }
+}
+
+// Both gradients in one launch: the first chunks of columns are dA's.
+template <typename T, int RB, OuterWork WORK>
+__global__ void __launch_bounds__(256)
+    adapter_outer_kernel(OuterSide<T> da, OuterSide<T> db, Plan p,
+                         int zstride, int R) {
+  __shared__ f32x4 part[2][RB * Vec<T>::N][WAVE];
+  __shared__ int list[SMALL_ROWS];
+  __shared__ int found;
+  const int column = blockIdx.x;
+  if (column < da.chunks)
+    outer_block<T, RB, true, WORK>(da, p, zstride, R, column, part, list,
+                                   found);
+  else
+    outer_block<T, RB, false, WORK>(db, p, zstride, R, column - da.chunks,
+                                    part, list, found);
 }
 
 // out_e = the sum of adapter e's partial sums, in their order; zero for an
 // adapter without rows.
 template <typename T>
 __global__ void __launch_bounds__(256)
-    adapter_reduce_kernel(const float* __restrict__ partial, Plan p,
-                          T* __restrict__ out, long n, int stretch) {
+    adapter_reduce_kernel(OuterSide<T> da, OuterSide<T> db, Plan p, int R) {
+  const OuterSide<T>& side = blockIdx.z == 0 ? da : db;
+  const long n = side.chunks ? (long)side.K * R : 0;
   const int e = blockIdx.y;
   const int tiles = p.tbase[e + 1] - p.tbase[e];
-  const int slots = (tiles + stretch - 1) / stretch;
-  const float* from = partial + (long)first_slot(p, e, stretch) * n;
+  const int slots = (tiles + side.stretch - 1) / side.stretch;
+  const float* from = side.partial + (long)first_slot(p, e, side.stretch) * n;
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n;
        i += (long)gridDim.x * 256) {
     float sum = 0.0f;
     for (int s = 0; s < slots; ++s) sum += from[s * n + i];
-    out[e * n + i] = (T)sum;
+    side.out[e * n + i] = (T)sum;
   }
 }
 
@@ -1081,17 +1121,19 @@ static float* check_z(const torch::Tensor& z, const torch::Tensor& like,
                       long M, long R) {
   TORCH_CHECK(R >= 1 && R <= RANK_MAX, "rank must be 1 .. 128");
   TORCH_CHECK(z.device() == like.device() && z.is_contiguous() &&
-                  z.scalar_type() == torch::kFloat32 && z.dim() == 2 &&
-                  z.size(0) == M && z.size(1) == padded_rank(R),
+                  z.scalar_type() == torch::kFloat32 && z.dim() == 3 &&
+                  z.size(0) >= 1 && z.size(1) == M &&
+                  z.size(2) == padded_rank(R),
               "z must be what adapter_shrink gave");
   return z.data_ptr<float>();
 }
 
-// z [M, Rp]: x [M, K] through w, [E, R, K] (kmajor) or [E, K, R].
+// z [planes, M, Rp], whose sum is x [M, K] through w, [E, R, K] (kmajor) or
+// [E, K, R].  More than one plane only where split allows it.
 torch::Tensor adapter_shrink(torch::Tensor x, torch::Tensor w,
                              torch::Tensor ids, torch::Tensor plan,
                              c10::optional<torch::Tensor> scales,
-                             double scale, bool kmajor) {
+                             double scale, bool kmajor, bool split) {
   const long M = x.size(0), E = w.size(0);
   check_weight(w, E);
   const long R = kmajor ? w.size(1) : w.size(2);
@@ -1111,11 +1153,17 @@ torch::Tensor adapter_shrink(torch::Tensor x, torch::Tensor w,
     sp = scales->data_ptr<float>();
   }
   const at::cuda::CUDAGuard guard(x.device());
-  auto z = torch::empty({M, padded_rank(R)},
+  const bool small = M <= SMALL_ROWS;
+  // Few rows: blocks of 4 waves for 16 KB of each row's adapter at a time,
+  // so that reading it is spread over the chip (32 rows of 4096 bf16, as
+  // many adapters: 4.9 us with 8 planes, 7.7 with one block of 16 waves).
+  const long bite = 4 * 4 * 64 / x.element_size() * 4;
+  const long planes =
+      small && split ? std::max<long>(1, std::min<long>(16, K / bite)) : 1;
+  auto z = torch::empty({planes, M, padded_rank(R)},
                         x.options().dtype(torch::kFloat32));
   if (M == 0) return z;
   auto stream = at::cuda::getCurrentCUDAStream();
-  const bool small = M <= SMALL_ROWS;
   for_dtype(x.scalar_type(), "x", [&](auto t) {
     using T = decltype(t);
     for_rank(R, [&](auto rb) {
@@ -1127,14 +1175,17 @@ torch::Tensor adapter_shrink(torch::Tensor x, torch::Tensor w,
       constexpr int U = RB == 1 ? 8 : RB == 2 ? 4 : 2;
       constexpr int MANY = RB <= 4 ? 16 : 8;  // waves whose sums fit the LDS
       auto go = [&](auto kernel, int waves, long blocks) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks),
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, (unsigned)planes),
                            dim3(waves * WAVE), 0, stream, ptr<T>(x),
                            (long)x.stride(0), ptr<T>(w), p, sp, (float)scale,
                            z.data_ptr<float>(), (int)K, (int)R);
       };
       auto pick = [&](auto major) {
         constexpr bool KM = decltype(major)::value;
-        if (small)
+        if (planes > 1)
+          go(adapter_shrink_kernel<T, RB, KM, true, 4, 1, RB <= 2 ? 4 : 2>, 4,
+             M);
+        else if (small)
           go(adapter_shrink_kernel<T, RB, KM, true, MANY, 1, U>, MANY, M);
         else if (M >= 4096 && (RB == 2 || RB == 4))
           go(adapter_shrink_kernel<T, RB, KM, false, 8, RB <= 4 ? 2 : 1,
@@ -1159,13 +1210,14 @@ torch::Tensor adapter_expand(c10::optional<torch::Tensor> base,
                              torch::Tensor z, torch::Tensor w,
                              torch::Tensor ids, torch::Tensor plan,
                              int64_t act, bool rmajor) {
-  const long M = z.size(0), E = w.size(0);
+  const long M = z.size(1), E = w.size(0);
   check_weight(w, E);
   const long N = rmajor ? w.size(1) : w.size(2);
   const long R = rmajor ? w.size(2) : w.size(1);
   TORCH_CHECK(N >= 1 && N < (1l << 30), "outputs must be 1 .. 2^30");
   const float* zp = check_z(z, w, M, R);
   if (base.has_value()) check_rows(*base, "base", M, N, w);
+  TORCH_CHECK(z.size(0) == 1 || M <= SMALL_ROWS, "z: one plane");
   const Plan p = plan_of(ids, plan, E);
   TORCH_CHECK(p.M == M && ids.device() == w.device(),
               "ids must be one a row beside the adapters");
@@ -1192,7 +1244,8 @@ torch::Tensor adapter_expand(c10::optional<torch::Tensor> base,
             dim3(waves * WAVE), 0, stream,
             base.has_value() ? ptr<T>(*base) : nullptr,
             base.has_value() ? (long)base->stride(0) : 0l, zp, ptr<T>(w), p,
-            ptr<T>(out), (int)N, (int)R, (int)act, (int)across);
+            ptr<T>(out), (int)N, (int)R, (int)act, (int)across,
+            (int)z.size(0));
       };
       if (rmajor && small)
         go(adapter_expand_kernel<T, RB, true, 1>, 1);
@@ -1208,39 +1261,65 @@ torch::Tensor adapter_expand(c10::optional<torch::Tensor> base,
   return out;
 }
 
-// [E, R, K] (kmajor) or [E, K, R]: the sums of z^T x over each adapter's
-// rows.
-torch::Tensor adapter_outer(torch::Tensor x, torch::Tensor z,
-                            torch::Tensor ids, torch::Tensor plan, int64_t E,
-                            int64_t R, bool kmajor) {
-  const long M = z.size(0), K = x.size(1);
-  check_rows(x, "x", M, K, x);
-  TORCH_CHECK(K >= 1 && K < (1l << 30), "inputs must be 1 .. 2^30");
-  const float* zp = check_z(z, x, M, R);
+// dA [E, R, K] = the sums of dz^T x over each adapter's rows, and dB
+// [E, N, R] those of dy^T z; either without its rows is not wanted.
+std::vector<torch::Tensor> adapter_outer(c10::optional<torch::Tensor> x,
+                                         c10::optional<torch::Tensor> dz,
+                                         c10::optional<torch::Tensor> dy,
+                                         c10::optional<torch::Tensor> z,
+                                         torch::Tensor ids,
+                                         torch::Tensor plan, int64_t E,
+                                         int64_t R) {
+  const c10::optional<torch::Tensor> from[2] = {x, dy}, of[2] = {dz, z};
+  TORCH_CHECK(x.has_value() || dy.has_value(), "nothing is wanted");
+  const torch::Tensor& like = x.has_value() ? *x : *dy;
   const Plan p = plan_of(ids, plan, E);
-  TORCH_CHECK(p.M == M && ids.device() == x.device(),
-              "ids must be one a row beside x");
-  const at::cuda::CUDAGuard guard(x.device());
-  auto out = kmajor ? torch::empty({E, R, K}, x.options())
-                    : torch::empty({E, K, R}, x.options());
+  TORCH_CHECK(ids.device() == like.device(), "ids must be beside x");
+  const long M = p.M;
+  const at::cuda::CUDAGuard guard(like.device());
   auto stream = at::cuda::getCurrentCUDAStream();
-  const long tiles = max_tiles(M, E);
   // Up to 1024 rows one block adds all of an adapter's; above, stretches
   // that give about 512 blocks, so that one busy adapter is not one block
   // (8192 rows of 4096 fp16: 44 us, with 256 blocks 54); in bf16, whose
   // products take less time than its rows' loads, 256 (22 us, with 512 24).
   const bool small = M <= SMALL_ROWS, direct = M <= 1024;
-  const long cols = 16 * (x.element_size() == 4 ? 4 : 8);
-  const long chunks = (K + cols - 1) / cols;
-  const long wanted = x.scalar_type() == torch::kBFloat16 ? 256 : 512;
-  const long stretch =
-      direct ? 1 : std::max<long>(4, M / TILE * chunks / wanted);
-  const long slots = direct ? E : tiles / stretch + E;
-  torch::Tensor partial;
-  if (!direct)
-    partial = torch::empty({slots, R, K}, x.options().dtype(torch::kFloat32));
-  for_dtype(x.scalar_type(), "x", [&](auto t) {
+  const long wanted = like.scalar_type() == torch::kBFloat16 ? 256 : 512;
+  const long cols = 16 * (like.element_size() == 4 ? 4 : 8);
+  std::vector<torch::Tensor> out(2), partial(2);
+  long stretch[2] = {1, 1}, chunks[2] = {0, 0}, K[2] = {0, 0}, slots = E;
+  const auto f32 = like.options().dtype(torch::kFloat32);
+  for (int i = 0; i < 2; ++i) {
+    if (!from[i].has_value()) continue;
+    K[i] = from[i]->size(1);
+    check_rows(*from[i], "rows", M, K[i], like);
+    TORCH_CHECK(K[i] >= 1 && K[i] < (1l << 30), "rows must be 1 .. 2^30 wide");
+    TORCH_CHECK(of[i].has_value() && of[i]->size(0) == 1, "z: one plane");
+    check_z(*of[i], like, M, R);
+    out[i] = torch::empty(i == 0 ? at::IntArrayRef({E, R, K[i]})
+                                 : at::IntArrayRef({E, K[i], R}),
+                          like.options());
+    chunks[i] = (K[i] + cols - 1) / cols;
+    if (direct) continue;
+    stretch[i] = std::max<long>(4, M / TILE * chunks[i] / wanted);
+    const long n = max_tiles(M, E) / stretch[i] + E;
+    partial[i] = torch::empty({n, R, K[i]}, f32);
+    slots = std::max(slots, n);
+  }
+  for_dtype(like.scalar_type(), "rows", [&](auto t) {
     using T = decltype(t);
+    OuterSide<T> side[2] = {};
+    for (int i = 0; i < 2; ++i) {
+      side[i].stretch = (int)stretch[i];
+      if (!from[i].has_value()) continue;
+      side[i] = {ptr<T>(*from[i]),
+                 (long)from[i]->stride(0),
+                 of[i]->data_ptr<float>(),
+                 ptr<T>(out[i]),
+                 direct ? nullptr : partial[i].data_ptr<float>(),
+                 (int)K[i],
+                 (int)chunks[i],
+                 (int)stretch[i]};
+    }
     for_rank(R, [&](auto rb) {
       // ranks above 32 take turns of 32: more sums than that do not fit
       // the registers beside their operands
@@ -1248,35 +1327,25 @@ torch::Tensor adapter_outer(torch::Tensor x, torch::Tensor z,
       auto go = [&](auto kernel) {
         hipLaunchKernelGGL(
             kernel,
-            dim3((unsigned)chunks, (unsigned)slots,
+            dim3((unsigned)(chunks[0] + chunks[1]), (unsigned)slots,
                  (unsigned)(padded_rank(R) / (16 * RB))),
-            dim3(256), 0, stream, ptr<T>(x), (long)x.stride(0), zp,
-            (int)z.size(1), p, ptr<T>(out),
-            direct ? nullptr : partial.data_ptr<float>(), (int)K, (int)R,
-            (int)stretch);
+            dim3(256), 0, stream, side[0], side[1], p, (int)padded_rank(R),
+            (int)R);
       };
-      auto pick = [&](auto major) {
-        constexpr bool KM = decltype(major)::value;
-        if (small)
-          go(adapter_outer_kernel<T, RB, KM, SMALL_OUTER>);
-        else if (direct)
-          go(adapter_outer_kernel<T, RB, KM, DIRECT_OUTER>);
-        else
-          go(adapter_outer_kernel<T, RB, KM, SPLIT_OUTER>);
-      };
-      if (kmajor)
-        pick(std::true_type());
+      if (small)
+        go(adapter_outer_kernel<T, RB, SMALL_OUTER>);
+      else if (direct)
+        go(adapter_outer_kernel<T, RB, DIRECT_OUTER>);
       else
-        pick(std::false_type());
+        go(adapter_outer_kernel<T, RB, SPLIT_OUTER>);
     });
     LAUNCH_OK();
     if (!direct) {
-      const long n = R * K;
+      const long n = R * std::max(K[0], K[1]);
       hipLaunchKernelGGL((adapter_reduce_kernel<T>),
                          dim3((unsigned)std::min<long>(256, (n + 255) / 256),
-                              (unsigned)E),
-                         dim3(256), 0, stream, partial.data_ptr<float>(), p,
-                         ptr<T>(out), n, (int)stretch);
+                              (unsigned)E, 2),
+                         dim3(256), 0, stream, side[0], side[1], p, (int)R);
       LAUNCH_OK();
     }
   });

@@ -94,7 +94,8 @@ struct AdapterAdd : public Function<AdapterAdd> {
   static Tensor forward(AutogradContext* ctx, Tensor base, Tensor x, Tensor a,
                         Tensor b, c10::optional<Tensor> scales, Tensor ids,
                         Tensor plan, double scale, int64_t act) {
-    const Tensor z = adapter_shrink(x, a, ids, plan, scales, scale, true);
+    const Tensor z =
+        adapter_shrink(x, a, ids, plan, scales, scale, true, false);
     const Tensor y = adapter_expand(base, z, b, ids, plan, act, true);
     ctx->save_for_backward(
         {x, a, b, z, scales.has_value() ? *scales : Tensor(), ids, plan,
@@ -111,6 +112,7 @@ struct AdapterAdd : public Function<AdapterAdd> {
     const int64_t act = ctx->saved_data["act"].toInt();
     const bool need_x = ctx->needs_input_grad(1);
     const bool need_a = ctx->needs_input_grad(2);
+    const bool need_b = ctx->needs_input_grad(3);
     Tensor dy, dx, da, db;
     {
       NoGrad none;
@@ -119,12 +121,18 @@ struct AdapterAdd : public Function<AdapterAdd> {
       Tensor dz;
       if (need_x || need_a)
         dz = adapter_shrink(dy, b, ids, plan, given(s[4]),
-                            ctx->saved_data["scale"].toDouble(), false);
+                            ctx->saved_data["scale"].toDouble(), false, false);
       if (need_x)
         dx = adapter_expand(c10::nullopt, dz, a, ids, plan, 0, false);
-      if (need_a) da = adapter_outer(x, dz, ids, plan, E, R, true);
-      if (ctx->needs_input_grad(3))
-        db = adapter_outer(dy, z, ids, plan, E, R, false);
+      if (need_a || need_b) {
+        const auto none = c10::optional<Tensor>();
+        const auto d = adapter_outer(
+            need_a ? given(x) : none, need_a ? given(dz) : none,
+            need_b ? given(dy) : none, need_b ? given(z) : none, ids, plan, E,
+            R);
+        da = d[0];
+        db = d[1];
+      }
     }
     const variable_list from = {g[0], x, a, b};
     Tensor dbase;
@@ -168,9 +176,18 @@ Tensor adapter_add_apply(Tensor base, Tensor x, Tensor a, Tensor b,
                          Tensor ids, c10::optional<Tensor> plan,
                          int64_t act) {
   const Tensor rows = ids.reshape(-1).contiguous();
-  const Tensor y = AdapterAdd::apply(
-      rows_of(base, b.size(1)), rows_of(x, a.size(2)), a.contiguous(),
-      b.contiguous(), scales, rows,
-      plan.has_value() ? *plan : adapter_plan(rows, a.size(0)), scale, act);
+  const Tensor base2 = rows_of(base, b.size(1)), x2 = rows_of(x, a.size(2));
+  const Tensor a2 = a.contiguous(), b2 = b.contiguous();
+  const Tensor p = plan.has_value() ? *plan : adapter_plan(rows, a.size(0));
+  Tensor y;
+  if (torch::GradMode::is_enabled() &&
+      (base.requires_grad() || x.requires_grad() || a.requires_grad() ||
+       b.requires_grad())) {
+    y = AdapterAdd::apply(base2, x2, a2, b2, scales, rows, p, scale, act);
+  } else {
+    const Tensor z =
+        adapter_shrink(x2, a2, rows, p, scales, scale, true, true);
+    y = adapter_expand(base2, z, b2, rows, p, act, true);
+  }
   return base.dim() == 2 ? y : y.reshape(base.sizes());
 }

@@ -28,14 +28,18 @@ torch::Tensor adapter_plan(torch::Tensor ids, int64_t E);
 torch::Tensor adapter_shrink(torch::Tensor x, torch::Tensor w,
                              torch::Tensor ids, torch::Tensor plan,
                              c10::optional<torch::Tensor> scales,
-                             double scale, bool kmajor);
+                             double scale, bool kmajor, bool split);
 torch::Tensor adapter_expand(c10::optional<torch::Tensor> base,
                              torch::Tensor z, torch::Tensor w,
                              torch::Tensor ids, torch::Tensor plan,
                              int64_t act, bool rmajor);
-torch::Tensor adapter_outer(torch::Tensor x, torch::Tensor z,
-                            torch::Tensor ids, torch::Tensor plan, int64_t E,
-                            int64_t R, bool kmajor);
+std::vector<torch::Tensor> adapter_outer(c10::optional<torch::Tensor> x,
+                                         c10::optional<torch::Tensor> dz,
+                                         c10::optional<torch::Tensor> dy,
+                                         c10::optional<torch::Tensor> z,
+                                         torch::Tensor ids,
+                                         torch::Tensor plan, int64_t E,
+                                         int64_t R);
 torch::Tensor adapter_act_bwd(torch::Tensor y, torch::Tensor dy,
                               int64_t act);
 
