@@ -954,6 +954,8 @@ def adapter_add(base, x, a, b, ids, scale=1.0, act="none"):
     b; an adapter that no row uses has a gradient of zero.
     """
     act = ACT_CODES[act] if isinstance(act, str) else act
+    if act not in (ACT_NONE, ACT_RELU, ACT_SIGMOID):
+        raise ValueError("unknown activation code %r" % (act,))
     tensors = (("base", base), ("x", x), ("a", a), ("b", b))
     for name, t in tensors:
         _check_float(name, t)

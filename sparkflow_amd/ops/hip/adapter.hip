@@ -1154,10 +1154,11 @@ torch::Tensor adapter_shrink(torch::Tensor x, torch::Tensor w,
   }
   const at::cuda::CUDAGuard guard(x.device());
   const bool small = M <= SMALL_ROWS;
-  // Few rows: blocks of 4 waves for 16 KB of each row's adapter at a time,
-  // so that reading it is spread over the chip (32 rows of 4096 bf16, as
-  // many adapters: 4.9 us with 8 planes, 7.7 with one block of 16 waves).
-  const long bite = 4 * 4 * 64 / x.element_size() * 4;
+  // Few rows: split along k, so that reading the adapters is spread over the
+  // chip.  32 rows of 4096 bf16 with as many adapters, shrink and expand
+  // together: 12.5 us with one plane, 10.5 with 2, 9.9 with 4 or 8 (expand
+  // has to add them), 10.9 with 16.
+  const long bite = 2048 / x.element_size();
   const long planes =
       small && split ? std::max<long>(1, std::min<long>(16, K / bite)) : 1;
   auto z = torch::empty({planes, M, padded_rank(R)},

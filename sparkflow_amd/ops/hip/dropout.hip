@@ -148,5 +148,7 @@ torch::Tensor dropout_next(torch::Tensor state) {
                      at::cuda::getCurrentCUDAStream(),
                      state.data_ptr<int64_t>(), out.data_ptr<int64_t>());
   LAUNCH_OK();
+  // a change in place, which autograd has to notice in what it saved
+  state.unsafeGetTensorImpl()->bump_version();
   return out;
 }

@@ -22,6 +22,8 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <climits>
+
 #include "vec.h"
 
 #define TOP_MAX 32
@@ -199,8 +201,11 @@ struct Tokens {
   long ignore;
 };
 
+// A NaN is no token (the conversion would make it 0).
 __device__ __forceinline__ long token_of(const Tokens& t, long row) {
-  return t.i64 ? t.i64[row] : (long)t.f32[row];
+  if (t.i64) return t.i64[row];
+  const float x = t.f32[row];
+  return x == x ? (long)x : LONG_MIN;
 }
 
 struct RowOut {

@@ -289,6 +289,7 @@ def test_adapter_add_refuses():
             F.adapter_groups(ids, e)
     with pytest.raises(KeyError):
         F.adapter_add(base, x, a, b, ids, act="tanh")
+    refused("activation code", act=3)
 
 
 # -- modules and models -------------------------------------------------------

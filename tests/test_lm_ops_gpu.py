@@ -345,6 +345,17 @@ def test_logprobs_token_types():
     assert other.logp[1] == 0 and torch.isnan(other.logp[2])
 
 
+def test_logprobs_labels_that_are_no_numbers():
+    """fp32 labels of NaN or an infinity name no class."""
+    logits = _randn(4, 9, seed=19)
+    labels = torch.tensor([math.nan, math.inf, -math.inf, 2.0], device=DEV)
+    r = F.token_logprobs(logits, labels, top_k=2)
+    assert torch.isnan(r.logp).tolist() == [True, True, True, False]
+    assert torch.isfinite(r.entropy).all() and (r.top_ids >= 0).all()
+    cpu = F.token_logprobs(logits.cpu(), labels.cpu(), top_k=2)
+    assert torch.isnan(cpu.logp).tolist() == [True, True, True, False]
+
+
 def test_logprobs_no_rows():
     x = torch.empty(0, 50, device=DEV, requires_grad=True)
     r = F.token_logprobs(x, torch.empty(0, dtype=torch.int64, device=DEV),
@@ -711,7 +722,7 @@ def test_changed_inputs_are_noticed():
     state = F.dropout_state(1, device=DEV)
     x = _randn(8).requires_grad_()
     y = F.dropout(x, 0.5, state)
-    state.add_(1)
+    F.dropout_next(state)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         y.sum().backward()
     base, x, a, b, ids, scale = _adapter_inputs(9, 8, 7, 2, 2)
