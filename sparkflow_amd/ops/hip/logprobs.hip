@@ -34,10 +34,12 @@ struct Stat {
   float m, s, t;
 };
 
-// The set moved to the larger maximum m.
+// The set moved to the larger maximum m.  The distance is bounded where its
+// exponential has long been 0: a set of nothing but the type's lowest value
+// would make s d infinite, and 0 times that NaN.
 __device__ __forceinline__ Stat stat_at(Stat a, float m) {
   if (a.m == m || a.m == -INFINITY) return {m, a.s, a.t};
-  const float d = a.m - m;
+  const float d = fmaxf(a.m - m, -1000.0f);
   const float f = __expf(d);
   return {m, a.s * f, (a.t + a.s * d) * f};
 }

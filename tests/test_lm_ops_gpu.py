@@ -236,6 +236,24 @@ def test_logprobs_masks(dtype, c):
     _check_logprobs(logits, tokens, 0)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("c", [300, 5000, 50001])
+def test_logprobs_masked_stretch(dtype, c):
+    """Threads, and whole splits, that hold nothing but the lowest value."""
+    logits = _randn(6, c, dtype=dtype, seed=14, std=4.0)
+    low = torch.finfo(dtype).min
+    logits[0, c // 3:] = low
+    logits[1, : c - 2] = low
+    logits[2, 40:] = low
+    logits[3, 1:] = -low         # one far below the others
+    logits[4, 7:] = low
+    logits[4, :7] = -math.inf
+    logits[5, c // 2:] = low / 2
+    tokens = torch.tensor([3, c - 1, 39, 2, 9, 1], device=DEV)
+    _check_logprobs(logits, tokens, 20)
+    _check_logprobs(logits, tokens, 0)
+
+
 @pytest.mark.parametrize("grads", [(1, 0, 0), (0, 1, 0), (0, 0, 1),
                                    (1, 0, 1)])
 def test_logprobs_single_gradients(grads):
