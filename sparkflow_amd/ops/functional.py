@@ -910,7 +910,7 @@ def _adapter_rows(ids, adapters, scales, scale):
 def _adapter_cpu(base, x, a, b, scales, scale, ids, act):
     f32 = torch.float32
     y = base.to(f32).clone()
-    z = torch.zeros(x.shape[0], a.shape[1])
+    z = torch.zeros(x.shape[0], a.shape[1], dtype=f32)
     for e, rows, s in _adapter_rows(ids, len(a), scales, scale):
         z[rows] = s * (x[rows].to(f32) @ a[e].to(f32).t())
         y[rows] += z[rows] @ b[e].to(f32).t()
@@ -922,7 +922,7 @@ def _adapter_grad_cpu(x, a, b, z, scales, ids, y, dy, scale, act):
     f32 = torch.float32
     if act != ACT_NONE:
         dy = _act_bwd_from_out(y.to(f32), dy.to(f32), act).to(dy.dtype)
-    dx, da, db = (torch.zeros(t.shape) for t in (x, a, b))
+    dx, da, db = (torch.zeros(t.shape, dtype=f32) for t in (x, a, b))
     for e, rows, s in _adapter_rows(ids, len(a), scales, scale):
         g = dy[rows].to(f32)
         dz = s * (g @ b[e].to(f32))
@@ -942,7 +942,7 @@ def adapter_add(base, x, a, b, ids, scale=1.0, act="none"):
     last axis lies side by side.  a: [adapters, rank, inputs], b: [adapters,
     outputs, rank], all in one type of fp32, bf16 or fp16; sums are 32 bits
     wide and every result is rounded once.  rank is at most 128, adapters
-    1024.
+    1024; on a GPU rows are less than 2^26.
 
     ids: one whole number a row (the leading shape of x), or the
     ``adapter_groups`` of them, which the layers of a model share.  A
@@ -951,7 +951,9 @@ def adapter_add(base, x, a, b, ids, scale=1.0, act="none"):
     the row is NaN, and so is its gradient of x.
 
     scale: a number, or fp32 [adapters].  Gradients flow to base, x, a and
-    b; an adapter that no row uses has a gradient of zero.
+    b; an adapter that no row uses has a gradient of zero.  What is not
+    finite in a row or an adapter stays within the rows and the gradients
+    that depend on it (an infinity there may come out as NaN).
     """
     act = ACT_CODES[act] if isinstance(act, str) else act
     if act not in (ACT_NONE, ACT_RELU, ACT_SIGMOID):

@@ -29,6 +29,8 @@
 #define TILE 16
 #define RANK_MAX 128
 #define ADAPTERS_MAX 1024
+// so that no launch has 2^32 threads: 512 for each tile
+#define ROWS_MAX (1l << 26)
 
 // -- rows by adapter ----------------------------------------------------------
 
@@ -727,13 +729,6 @@ __device__ __forceinline__ int first_slot(const Plan& p, int e,
   return p.tbase[e] / stretch + e;
 }
 
-// sum over the rows of a stretch of one adapter: z[place][r] x[row][k].  A
-// lane loads 16 bytes of a row; instruction j takes element j of all lanes,
-// so its 16 columns are k0 + V (l % 16) + j.  Its sum runs over four rows in
-// fp32; in bf16 over 32, of which a lane has every fourth: eight loads, whose
-// elements j are one operand, beside z in three parts.  KMAJOR: the result is [R, K] (dA), else [K, R]
-// (dB).  SMALL_OUTER, DIRECT_OUTER: one block an adapter, rounded into out;
-// SPLIT_OUTER: one block a stretch, into fp32 sums that reduce joins.
 // One of the two: dA from x and dz, or dB from dy and z.
 template <typename T>
 struct OuterSide {
@@ -745,6 +740,14 @@ struct OuterSide {
   int K, chunks, stretch;  // chunks of 16 V columns; 0: not wanted
 };
 
+// sum over the rows of a stretch of one adapter: z[place][r] x[row][k].  A
+// lane loads 16 bytes of a row; instruction j takes element j of all lanes,
+// so its 16 columns are k0 + V (l % 16) + j.  Its sum runs over four rows in
+// fp32; in bf16 over 32, of which a lane has every fourth: eight loads, whose
+// elements j are one operand, beside z in three parts.  KMAJOR: the result
+// is [R, K] (dA), else [K, R] (dB).  SMALL_OUTER, DIRECT_OUTER: one block an
+// adapter, rounded into out; SPLIT_OUTER: one block a stretch, into fp32
+// sums that reduce joins.
 template <typename T, int RB, bool KMAJOR, OuterWork WORK>
 __device__ __forceinline__ void outer_block(
     const OuterSide<T>& side, const Plan& p, int zstride, int R, int column,
@@ -775,7 +778,7 @@ __device__ __forceinline__ void outer_block(
     for (int e = threadIdx.x; e < p.E; e += 256) {
       const int c = (int)blockIdx.y - first_slot(p, e, stretch);
       const int n = p.tbase[e + 1] - p.tbase[e];
-      if (c >= 0 && c * stretch < n) {
+      if (c >= 0 && (long)c * stretch < n) {
         found = e;
         list[0] = p.seg[e] + c * stretch * TILE;
       }
@@ -790,78 +793,79 @@ __device__ __forceinline__ void outer_block(
   const int k = k0 + i * V;
   f32x4 acc[RB][V] = {};
   // The bf16 loop: 32 rows a step.  Nothing but the rows' numbers is loaded
-  // a step ahead: the registers go into a third wave a SIMD instead.
+  // a step ahead: with the rows too the loop took 268 registers, one wave a
+  // SIMD, for 204, two (dA of 8192 rows x 4096: 34.9 us for 24.4).
   auto steps32 = [&](auto whole) {
     if constexpr (BF16) {
-    constexpr bool WHOLE = decltype(whole)::value;
-    constexpr int STEP = 4 * 32;  // of the four waves
-    int row[U];
-    auto place = [&](int m0, int u) {
-      const int at = min(m0 + 4 * u + quarter, end - 1);
-      return WORK == SMALL_OUTER ? list[at] : at;
-    };
-    auto number = [&](int m0) {
+      constexpr bool WHOLE = decltype(whole)::value;
+      constexpr int STEP = 4 * 32;  // of the four waves
+      int row[U];
+      auto place = [&](int m0, int u) {
+        const int at = min(m0 + 4 * u + quarter, end - 1);
+        return WORK == SMALL_OUTER ? list[at] : at;
+      };
+      auto number = [&](int m0) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        row[u] = WORK == SMALL_OUTER ? place(m0, u) : p.perm[place(m0, u)];
-    };
-    int m0 = begin + wave * 32;
-    if (m0 < end) number(m0);
-    for (; m0 < end; m0 += STEP) {
-      typename Vec<T>::V xv[U];
-      float zv[RB][U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const T* xr = x + (long)row[u] * xstride;
-        if (WHOLE) {
-          xv[u] = Vec<T>::load(xr + k);
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j)
-            xv[u][j] = k + j < K ? xr[k + j] : (T)0.0f;
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int c = 0; c < RB; ++c)
-          zv[c][u] = z[(long)place(m0, u) * zstride + r0 + 16 * c + i];
-      number(m0 + STEP);
-      if (m0 + 32 > end) {
-        // rows behind the last: both factors, since 0 x NaN is not 0
+        for (int u = 0; u < U; ++u)
+          row[u] = WORK == SMALL_OUTER ? place(m0, u) : p.perm[place(m0, u)];
+      };
+      int m0 = begin + wave * 32;
+      if (m0 < end) number(m0);
+      for (; m0 < end; m0 += STEP) {
+        typename Vec<T>::V xv[U];
+        float zv[RB][U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const bool in = m0 + 4 * u + quarter < end;
+          const T* xr = x + (long)row[u] * xstride;
+          if (WHOLE) {
+            xv[u] = Vec<T>::load(xr + k);
+          } else {
 #pragma unroll
-          for (int j = 0; j < V; ++j) xv[u][j] = in ? xv[u][j] : (T)0.0f;
-#pragma unroll
-          for (int c = 0; c < RB; ++c) zv[c][u] = in ? zv[c][u] : 0.0f;
-        }
-      }
-      Split zs[RB];
-#pragma unroll
-      for (int c = 0; c < RB; ++c) zs[c] = split(zv[c]);
-#pragma unroll
-      for (int j = 0; j < V; j += 2) {
-        typename Vec<T>::V col[2];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          col[0][u] = xv[u][j];
-          col[1][u] = xv[u][j + 1];
+            for (int j = 0; j < V; ++j)
+              xv[u][j] = k + j < K ? xr[k + j] : (T)0.0f;
+          }
         }
 #pragma unroll
-        for (int part = 0; part < 3; ++part)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
           for (int c = 0; c < RB; ++c)
+            zv[c][u] = z[(long)place(m0, u) * zstride + r0 + 16 * c + i];
+        number(m0 + STEP);
+        if (m0 + 32 > end) {
+          // rows behind the last: both factors, since 0 x NaN is not 0
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              acc[c][j + h] = mma(part == 0   ? zs[c].low
-                                  : part == 1 ? zs[c].mid
-                                              : zs[c].high,
-                                  col[h], acc[c][j + h]);
+          for (int u = 0; u < U; ++u) {
+            const bool in = m0 + 4 * u + quarter < end;
+#pragma unroll
+            for (int j = 0; j < V; ++j) xv[u][j] = in ? xv[u][j] : (T)0.0f;
+#pragma unroll
+            for (int c = 0; c < RB; ++c) zv[c][u] = in ? zv[c][u] : 0.0f;
+          }
+        }
+        Split zs[RB];
+#pragma unroll
+        for (int c = 0; c < RB; ++c) zs[c] = split(zv[c]);
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+          typename Vec<T>::V col[2];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            col[0][u] = xv[u][j];
+            col[1][u] = xv[u][j + 1];
+          }
+#pragma unroll
+          for (int part = 0; part < 3; ++part)
+#pragma unroll
+            for (int c = 0; c < RB; ++c)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                acc[c][j + h] = mma(part == 0   ? zs[c].low
+                                    : part == 1 ? zs[c].mid
+                                                : zs[c].high,
+                                    col[h], acc[c][j + h]);
+        }
       }
     }
-  }
   };
   // Four rows an instruction, U times four a step.  The next step's rows
   // are loaded before this one's products, and their numbers a step before
@@ -1059,8 +1063,8 @@ static Plan plan_of(const torch::Tensor& ids, const torch::Tensor& plan,
                     long E) {
   TORCH_CHECK(ids.is_cuda() && ids.is_contiguous() && ids.dim() == 1 &&
                   ids.scalar_type() == torch::kInt64 &&
-                  ids.size(0) < (1l << 28),
-              "ids must be contiguous int64 [rows] on GPU");
+                  ids.size(0) < ROWS_MAX,
+              "ids must be contiguous int64 [rows] on GPU, less than 2^26");
   TORCH_CHECK(E >= 1 && E <= ADAPTERS_MAX, "1 .. 1024 adapters");
   const long M = ids.size(0);
   TORCH_CHECK(plan.device() == ids.device() && plan.is_contiguous() &&
@@ -1155,7 +1159,7 @@ torch::Tensor adapter_shrink(torch::Tensor x, torch::Tensor w,
   const long K = kmajor ? w.size(2) : w.size(1);
   check_rows(x, "x", M, K, w);
   TORCH_CHECK(R >= 1 && R <= RANK_MAX, "rank must be 1 .. 128");
-  TORCH_CHECK(K >= 1 && K < (1l << 30), "inputs must be 1 .. 2^30");
+  TORCH_CHECK(K >= 1 && K < (1l << 28), "inputs must be 1 .. 2^28");
   const Plan p = plan_of(ids, plan, E);
   TORCH_CHECK(p.M == M && ids.device() == x.device(),
               "ids must be one a row beside x");
@@ -1230,7 +1234,7 @@ torch::Tensor adapter_expand(c10::optional<torch::Tensor> base,
   check_weight(w, E);
   const long N = rmajor ? w.size(1) : w.size(2);
   const long R = rmajor ? w.size(2) : w.size(1);
-  TORCH_CHECK(N >= 1 && N < (1l << 30), "outputs must be 1 .. 2^30");
+  TORCH_CHECK(N >= 1 && N < (1l << 28), "outputs must be 1 .. 2^28");
   const float* zp = check_z(z, w, M, R);
   if (base.has_value()) check_rows(*base, "base", M, N, w);
   TORCH_CHECK(z.size(0) == 1 || M <= SMALL_ROWS, "z: one plane");
@@ -1254,9 +1258,8 @@ torch::Tensor adapter_expand(c10::optional<torch::Tensor> base,
         const long chunks = (N + cols - 1) / cols;
         long turns = std::max<long>(1, chunks * blocks / 2048);
         const long across = (chunks + turns - 1) / turns;
-        TORCH_CHECK(blocks * across < (1l << 31), "too many rows");
         hipLaunchKernelGGL(
-            kernel, dim3((unsigned)(blocks * across)),
+            kernel, grid_of(blocks * across, waves * WAVE, "adapters"),
             dim3(waves * WAVE), 0, stream,
             base.has_value() ? ptr<T>(*base) : nullptr,
             base.has_value() ? (long)base->stride(0) : 0l, zp, ptr<T>(w), p,
@@ -1308,7 +1311,7 @@ std::vector<torch::Tensor> adapter_outer(c10::optional<torch::Tensor> x,
     if (!from[i].has_value()) continue;
     K[i] = from[i]->size(1);
     check_rows(*from[i], "rows", M, K[i], like);
-    TORCH_CHECK(K[i] >= 1 && K[i] < (1l << 30), "rows must be 1 .. 2^30 wide");
+    TORCH_CHECK(K[i] >= 1 && K[i] < (1l << 28), "rows must be 1 .. 2^28 wide");
     TORCH_CHECK(of[i].has_value() && of[i]->size(0) == 1, "z: one plane");
     check_z(*of[i], like, M, R);
     out[i] = torch::empty(i == 0 ? at::IntArrayRef({E, R, K[i]})

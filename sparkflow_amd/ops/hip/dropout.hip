@@ -122,10 +122,8 @@ torch::Tensor dropout(torch::Tensor x, torch::Tensor state, int64_t keep,
     using T = decltype(t);
     const long vecs = (n + Vec<T>::N - 1) / Vec<T>::N;
     auto go = [&](auto kernel) {
-      const long blocks = (vecs + 255) / 256;
-      TORCH_CHECK(blocks < (1l << 31), "dropout: tensor too large");
-      hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0,
-                         stream, ptr<T>(x), ptr<T>(y),
+      hipLaunchKernelGGL(kernel, grid_of((vecs + 255) / 256, 256, "dropout"),
+                         dim3(256), 0, stream, ptr<T>(x), ptr<T>(y),
                          state.data_ptr<int64_t>(), n,
                          (unsigned)(keep - 1), (float)scale);
     };

@@ -203,11 +203,12 @@ struct Tokens {
   long ignore;
 };
 
-// A NaN is no token (the conversion would make it 0).
+// What does not fit 64 bits, a NaN among it, is no token (the conversion
+// has no defined result).
 __device__ __forceinline__ long token_of(const Tokens& t, long row) {
   if (t.i64) return t.i64[row];
   const float x = t.f32[row];
-  return x == x ? (long)x : LONG_MIN;
+  return fabsf(x) < 0x1p62f ? (long)x : LONG_MIN;
 }
 
 struct RowOut {
@@ -720,7 +721,6 @@ std::vector<torch::Tensor> logprobs_fwd(torch::Tensor logits,
     long span = (C + splits - 1) / splits;
     span = (span + N - 1) / N * N;
     splits = (C + span - 1) / span;
-    TORCH_CHECK(M * splits < (1l << 31), "logits: too many rows");
     torch::Tensor pstat, pkeys;
     if (splits > 1) {
       pstat = torch::empty({M, splits, 3}, f32);
@@ -732,9 +732,9 @@ std::vector<torch::Tensor> logprobs_fwd(torch::Tensor logits,
                    : nullptr;
     const T* x = ptr<T>(logits);
     auto go = [&](auto kernel, int nt) {
-      hipLaunchKernelGGL(kernel, dim3((unsigned)(M * splits)), dim3(nt), 0,
-                         stream, x, (long)logits.stride(0), tok, out, ps, pk,
-                         C, (int)splits, span, (int)k);
+      hipLaunchKernelGGL(kernel, grid_of(M * splits, nt, "logits"), dim3(nt),
+                         0, stream, x, (long)logits.stride(0), tok, out, ps,
+                         pk, C, (int)splits, span, (int)k);
     };
     // One wave a row while a row gives a wave no more than 4 vectors a
     // lane; more rows are in flight then and nothing waits at a barrier.
@@ -797,11 +797,10 @@ torch::Tensor logprobs_bwd(torch::Tensor logits, torch::Tensor tokens,
     constexpr int N = Vec<T>::N;
     auto go = [&](auto kernel, int nt, long span) {
       const long spans = (C + span - 1) / span;
-      TORCH_CHECK(M * spans < (1l << 31), "logits: too many rows");
-      hipLaunchKernelGGL(kernel, dim3((unsigned)(M * spans)), dim3(nt), 0,
-                         stream, ptr<T>(logits), (long)logits.stride(0), tok,
-                         pl, pe, ids.data_ptr<int64_t>(), grad, ptr<T>(dx),
-                         C, (int)spans, span, k);
+      hipLaunchKernelGGL(kernel, grid_of(M * spans, nt, "logits"), dim3(nt),
+                         0, stream, ptr<T>(logits), (long)logits.stride(0),
+                         tok, pl, pe, ids.data_ptr<int64_t>(), grad,
+                         ptr<T>(dx), C, (int)spans, span, k);
     };
     if (C <= 4 * WAVE * N) {
       go(logprobs_bwd_kernel<T, 64>, 64, 4 * WAVE * N);

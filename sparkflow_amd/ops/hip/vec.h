@@ -55,6 +55,12 @@ static inline T* ptr(const torch::Tensor& t) {
   return reinterpret_cast<T*>(t.data_ptr());
 }
 
+// The blocks of a launch, whose threads are counted in 32 bits.
+static inline dim3 grid_of(long blocks, int threads, const char* name) {
+  TORCH_CHECK(blocks * threads < (1l << 32), name, ": too many rows");
+  return dim3((unsigned)blocks);
+}
+
 // After a launch: a refused launch becomes an exception at the call.
 #define LAUNCH_OK()                                                     \
   do {                                                                  \

@@ -374,6 +374,19 @@ def test_logprobs_labels_that_are_no_numbers():
     assert torch.isnan(cpu.logp).tolist() == [True, True, True, False]
 
 
+def test_more_rows_than_a_launch_has_are_refused():
+    """One row in memory, seen 2^26 times."""
+    m = 2 ** 26
+    ids = torch.zeros(m, dtype=torch.int64, device=DEV)
+    x = torch.zeros(1, 4, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(RuntimeError, match="too many rows"):
+        F.token_logprobs(x.expand(m, 4), ids)
+    a = torch.zeros(2, 1, 4, dtype=torch.bfloat16, device=DEV)
+    b = torch.zeros(2, 4, 1, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(RuntimeError, match="less than 2\\^26"):
+        F.adapter_add(x.expand(m, 4), x.expand(m, 4), a, b, ids)
+
+
 def test_logprobs_no_rows():
     x = torch.empty(0, 50, device=DEV, requires_grad=True)
     r = F.token_logprobs(x, torch.empty(0, dtype=torch.int64, device=DEV),
