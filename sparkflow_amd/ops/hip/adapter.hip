@@ -428,31 +428,30 @@ __global__ void __launch_bounds__(WAVES * WAVE)
   }
 }
 
-// The activations, a NaN staying one.
-__device__ __forceinline__ float act_keep_nan(float x, int act) {
-  if (act == ACT_RELU) return x < 0.0f ? 0.0f : x;
-  return act_apply(x, act);
-}
-
 // -- expand -------------------------------------------------------------------
 
 // out[row][n] = act(base[row][n] + sum_r z[place][r] W_e(n, r)), W [N, R]
-// (RMAJOR) or [R, N].  One block takes up to WAVES tiles of an adapter, a
-// wave a tile, through chunks of 16 V columns; a chunk's part of W is laid
-// into LDS as it lies in memory, and the loads of the next chunk are under
-// way during this one's products.  The product is taken as D[n][m], in
-// fp32; instruction j's row 4 h + q is the chunk's column
+// (RMAJOR), or without base and act, W [R, N].  One block takes up to WAVES
+// tiles of an adapter, a wave a tile, through chunks of 16 V columns; a
+// chunk's part of W is laid into LDS (in bf16 [R, N] is turned round there),
+// and the loads of the next chunk are under way during this one's products.
+// The product is taken as D[n][m], in fp32, or in bf16 with z in three parts;
+// instruction j's row 4 h + q is the chunk's column
 // 4 V a + V h + e, where j = a V / 4 + e / 4 and q = e % 4, so that a lane
 // ends up with 16 bytes of adjacent outputs and its row's four lanes with
 // 64.  base enters as the sum's first term.  8192 rows of 4096 bf16 at a rank
 // of 16 (base read, out written: 134 MB): 28.7 us, 4.7 TB/s; a plain copy
-// takes 21.
-template <typename T, int RB, bool RMAJOR, int WAVES>
+// takes 21.  What only one of the forms needs is left out of the others at
+// compile time: 32 divisions of a sigmoid and the base are registers of a
+// fourth wave a SIMD (out of 8192 rows of 4096 alone, 67 MB, at a rank of 32:
+// 21.1 us for 25.4).  Lanes that trade places, for 128 bytes of a
+// row an instruction, and 1024 or 4096 blocks measured no better.
+template <typename T, int RB, bool RMAJOR, bool SIGMOID, int WAVES>
 __global__ void __launch_bounds__(WAVES * WAVE)
     adapter_expand_kernel(const T* __restrict__ base, long bstride,
                           const float* __restrict__ z,
                           const T* __restrict__ w, Plan p,
-                          T* __restrict__ out, int N, int R, int act,
+                          T* __restrict__ out, int N, int R, bool relu,
                           int across, int planes) {
   constexpr int V = Vec<T>::N;
   constexpr int COLS = 16 * V;
@@ -507,7 +506,7 @@ __global__ void __launch_bounds__(WAVES * WAVE)
   // Only the last chunk has vectors to cut: the others load without
   // branches.
   auto load_base = [&](int n0) {
-    if (base == nullptr) return;
+    if (!RMAJOR) return;
     const int c0 = n0 + V * quarter;
     if (n0 + COLS <= N) {
 #pragma unroll
@@ -655,8 +654,7 @@ __global__ void __launch_bounds__(WAVES * WAVE)
       constexpr int H = V / 4;  // instructions to a vector of the output
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        acc[j][q] =
-            base != nullptr ? (float)bv[j / H][4 * (j % H) + q] : 0.0f;
+        acc[j][q] = RMAJOR ? (float)bv[j / H][4 * (j % H) + q] : 0.0f;
       if (adapted) {
         const int c = 4 * V * (j / H) + V * (i >> 2) + 4 * (j % H) + (i & 3);
         if constexpr (BF16) {
@@ -692,11 +690,18 @@ __global__ void __launch_bounds__(WAVES * WAVE)
     if (g > p.E) {
 #pragma unroll
       for (int j = 0; j < V; ++j) acc[j] = f32x4{NAN, NAN, NAN, NAN};
-    } else if (act != ACT_NONE) {
+    } else if (RMAJOR && relu) {
 #pragma unroll
       for (int j = 0; j < V; ++j)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) acc[j][q] = act_keep_nan(acc[j][q], act);
+        for (int q = 0; q < 4; ++q)
+          acc[j][q] = acc[j][q] < 0.0f ? 0.0f : acc[j][q];  // NaN stays
+    } else if (SIGMOID) {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          acc[j][q] = act_apply(acc[j][q], ACT_SIGMOID);
     }
     VT v[4];
 #pragma unroll
@@ -1225,7 +1230,7 @@ torch::Tensor adapter_shrink(torch::Tensor x, torch::Tensor w,
   return z;
 }
 
-// act(base + z w): w [E, N, R] (rmajor) or [E, R, N]; no base: zero.
+// act(base + z w) with w [E, N, R] (rmajor), or z w with w [E, R, N].
 torch::Tensor adapter_expand(c10::optional<torch::Tensor> base,
                              torch::Tensor z, torch::Tensor w,
                              torch::Tensor ids, torch::Tensor plan,
@@ -1237,6 +1242,8 @@ torch::Tensor adapter_expand(c10::optional<torch::Tensor> base,
   TORCH_CHECK(N >= 1 && N < (1l << 28), "outputs must be 1 .. 2^28");
   const float* zp = check_z(z, w, M, R);
   if (base.has_value()) check_rows(*base, "base", M, N, w);
+  TORCH_CHECK(base.has_value() == rmajor && (rmajor || act == ACT_NONE),
+              "a base and an activation belong to [outputs, rank]");
   TORCH_CHECK(z.size(0) == 1 || M <= SMALL_ROWS, "z: one plane");
   const Plan p = plan_of(ids, plan, E);
   TORCH_CHECK(p.M == M && ids.device() == w.device(),
@@ -1263,17 +1270,25 @@ torch::Tensor adapter_expand(c10::optional<torch::Tensor> base,
             dim3(waves * WAVE), 0, stream,
             base.has_value() ? ptr<T>(*base) : nullptr,
             base.has_value() ? (long)base->stride(0) : 0l, zp, ptr<T>(w), p,
-            ptr<T>(out), (int)N, (int)R, (int)act, (int)across,
+            ptr<T>(out), (int)N, (int)R, act == ACT_RELU, (int)across,
             (int)z.size(0));
       };
-      if (rmajor && small)
-        go(adapter_expand_kernel<T, RB, true, 1>, 1);
-      else if (rmajor)
-        go(adapter_expand_kernel<T, RB, true, 4>, 4);
-      else if (small)
-        go(adapter_expand_kernel<T, RB, false, 1>, 1);
+      auto pick = [&](auto major, auto sigmoid) {
+        constexpr bool RM = decltype(major)::value;
+        constexpr bool SG = decltype(sigmoid)::value;
+        if (small)
+          go(adapter_expand_kernel<T, RB, RM, SG, 1>, 1);
+        else
+          go(adapter_expand_kernel<T, RB, RM, SG, 4>, 4);
+      };
+      const std::true_type yes;
+      const std::false_type no;
+      if (!rmajor)
+        pick(no, no);
+      else if (act == ACT_SIGMOID)
+        pick(yes, yes);
       else
-        go(adapter_expand_kernel<T, RB, false, 4>, 4);
+        pick(yes, no);
     });
   });
   LAUNCH_OK();
