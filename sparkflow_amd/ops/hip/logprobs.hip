@@ -71,9 +71,12 @@ __device__ __forceinline__ Stat wave_join(Stat a) {
 // are what bounds the pass in the 16-bit types.  The sums move to another
 // shift only when a value is 2.5 above `ref`, where they were put last: some
 // lane of a wave has a new maximum almost every time, and seldom one that
-// far.  Two sums each, for shorter chains.  Where ref log2 e leaves fp32 (the
-// lowest value as a mask of a whole row) or is infinite, the sums are about
-// ref itself.
+// far.  Two sums each, for shorter chains.
+//
+// ref log2 e is rounded before it becomes a whole number, by half a step of
+// fp32: 1/16 at 2^20, but 512 at a mask of -1e10, whose exponential would be
+// infinite or 0.  From 2^20 on, and for an infinity, the sums are therefore
+// about ref itself.
 struct Run {
   float m, ref, limit, shift, s0, s1, t0, t1;
 
@@ -83,7 +86,7 @@ struct Run {
   }
 
   static __device__ __forceinline__ bool far(float ref) {
-    return !(fabsf(ref) < 1.0e38f);
+    return !(fabsf(ref) < 0x1p20f);
   }
 
   // Adds n values.
@@ -100,8 +103,11 @@ struct Run {
       shift = rintf(gm * LOG2E);
       limit = far(ref) ? ref : ref + 2.5f;
       if (old != -INFINITY) {
-        const float d =
-            far(old) || far(ref) ? (old - ref) * LOG2E : from - shift;
+        // from what the sums were about to what they are about now
+        const float d = far(old)   ? (far(ref) ? (old - ref) * LOG2E
+                                               : fmaf(old, LOG2E, -shift))
+                        : far(ref) ? -fmaf(ref, LOG2E, -from)
+                                   : from - shift;
         const float f = __builtin_amdgcn_exp2f(d);
         // a reference of infinite distance leaves nothing of the old sums
         const float g = fmaxf(d, -1000.0f);

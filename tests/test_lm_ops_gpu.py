@@ -254,6 +254,49 @@ def test_logprobs_masked_stretch(dtype, c):
     _check_logprobs(logits, tokens, 0)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mask", [-1e6, -1e9, -1e10, -1e15, -1e20, -1e30,
+                                  -1e37, 1e10, 1e30])
+@pytest.mark.parametrize("c", [48, 700, 5000, 50001])
+def test_logprobs_masks_of_any_size(dtype, mask, c):
+    """Finite masks between common logits and the type's lowest value."""
+    logits = _randn(9, c, dtype=dtype, seed=24, std=4.0)
+    n = 16 // dtype.itemsize
+    logits[0, n:2 * n] = mask               # all that one thread sees
+    logits[1, c // 3:] = mask
+    logits[2, : c - 2] = mask
+    logits[3] = mask
+    logits[4, ::2] = mask
+    logits[5, : c // 2] = -math.inf         # nothing else is possible
+    logits[5, c // 2:] = mask
+    logits[6, : c // 2] = torch.finfo(dtype).min
+    logits[6, c // 2:] = mask
+    logits[7, : c // 2] = 2 * mask          # one mask upon another
+    logits[7, c // 2:] = mask
+    logits[8, : c // 2] = mask
+    tokens = torch.tensor([0, 1, c - 1, 2, 3, c - 1, c - 2, c - 3, 5],
+                          device=DEV)
+    _check_logprobs(logits, tokens, 20)
+    _check_logprobs(logits, tokens, 0)
+
+
+@pytest.mark.parametrize("at", [2.0 ** 18, 2.0 ** 20, 2.0 ** 21, 2.0 ** 23,
+                                2.0 ** 24, 1e9, 1e12])
+@pytest.mark.parametrize("c", [1000, 20000])
+def test_logprobs_far_from_zero(c, at):
+    """Maxima that rise and fall about sizes where fp32 has few places, or
+    none, behind the point; rows long enough for several rounds a thread."""
+    ramp = torch.linspace(-4, 4, c, device=DEV)
+    logits = torch.zeros(512, c, device=DEV)
+    rows = [at + ramp, at - ramp, ramp - at, -ramp - at, ramp * at,
+            -ramp * at, ramp * (at / 4) - 2.0 ** 20]
+    for i, row in enumerate(rows):
+        logits[70 * i] = row
+    tokens = torch.full((512,), -100, device=DEV)
+    tokens[:70 * len(rows):70] = torch.arange(len(rows), device=DEV) + c // 2
+    _check_logprobs(logits, tokens, 5)
+
+
 @pytest.mark.parametrize("grads", [(1, 0, 0), (0, 1, 0), (0, 0, 1),
                                    (1, 0, 1)])
 def test_logprobs_single_gradients(grads):
