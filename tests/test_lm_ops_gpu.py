@@ -297,6 +297,25 @@ def test_logprobs_far_from_zero(c, at):
     _check_logprobs(logits, tokens, 5)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_logprobs_one_likely_class(dtype):
+    """No log-probability is above 0 and no entropy below."""
+    value = torch.linspace(-9, 9, 600, device=DEV)
+    tokens = torch.zeros(600, device=DEV)
+    for c in (1, 3, 64, 1000, 5000):
+        for rest in (-math.inf, -300.0):
+            logits = torch.full((600, c), rest, device=DEV)
+            logits[:, 0] = value
+            r = F.token_logprobs(logits.to(dtype), tokens, top_k=1)
+            for t in (r.logp, r.top_logp):
+                assert (t <= 0).all()
+                assert (t >= -oracle.logprobs_tol(
+                    torch.zeros(()), False, c)).all()
+            assert (r.entropy >= 0).all()
+            assert (r.entropy <= oracle.logprobs_tol(
+                torch.zeros(()), True, c)).all()
+
+
 @pytest.mark.parametrize("grads", [(1, 0, 0), (0, 1, 0), (0, 0, 1),
                                    (1, 0, 1)])
 def test_logprobs_single_gradients(grads):
