@@ -802,9 +802,13 @@ def token_logprobs(logits, tokens, top_k: int = 0,
     * A token outside 0 .. classes - 1 cannot be refused without waiting
       for the device: its log-probability is NaN, and so is its row of the
       gradient if one flows from there.
-    * A logit of -inf has probability 0, adds nothing to the entropy and
-      takes no gradient through it.  A row of nothing else has -inf for
-      every class, an entropy of 0 and a gradient of zero.
+    * A logit of -inf has probability 0 and adds nothing to the entropy; in
+      its gradient the probability's terms are 0.  What flows to a class
+      that is named, as the token or as an alternative, reaches its logit
+      all the same, as in a log-softmax: where fewer classes than ``top_k``
+      are possible, leave the impossible alternatives (a ``top_logp`` of
+      -inf) out of the loss.  A row of nothing else has -inf for every
+      class, an entropy of 0 and a gradient of zero.
     * A row that holds NaN or +inf has no distribution: NaN everywhere and
       top ids of -1.
     """

@@ -142,6 +142,32 @@ def test_logprobs_agrees_with_softmax_xent():
     torch.testing.assert_close(x.grad, y.grad)
 
 
+def check_gradient_of_impossible_classes(device):
+    """What flows to a named class reaches its logit, possible or not; the
+    others' probabilities are 0 and add nothing."""
+    rows = torch.tensor([[0.0, 1.0, -math.inf, -math.inf]] * 2)
+    tokens = torch.tensor([2, 0])
+    x = rows.to(device).requires_grad_()
+    r = F.token_logprobs(x, tokens.to(device), top_k=3)
+    assert r.logp.tolist()[0] == -math.inf
+    assert r.top_logp[:, 2].tolist() == [-math.inf] * 2
+    y = rows.double().requires_grad_()
+    logp = torch.log_softmax(y, 1)
+    for got, want in ((r.logp, logp.gather(1, tokens.unsqueeze(1))),
+                      (r.top_logp, logp.gather(1, r.top_ids.cpu())),
+                      (r.top_logp[:, :2], logp[:, :2])):
+        (dx,) = torch.autograd.grad(got.sum(), x, retain_graph=True)
+        (dy,) = torch.autograd.grad(want.sum(), y, retain_graph=True)
+        # four terms of size 3 at most, each a few half steps off
+        assert ((dx.cpu().double() - dy).abs() <= 64 * oracle.U32).all()
+    (dx,) = torch.autograd.grad(r.entropy.sum(), x)
+    assert (dx[:, 2:] == 0).all() and torch.isfinite(dx).all()
+
+
+def test_logprobs_gradient_of_impossible_classes():
+    check_gradient_of_impossible_classes("cpu")
+
+
 def test_logprobs_broken_rows_and_tokens():
     logits = torch.randn(5, 9)
     logits[1, 3] = math.nan

@@ -324,6 +324,12 @@ def test_logprobs_single_gradients(grads):
     _check_logprobs(logits, tokens, 4, grads=grads)
 
 
+def test_logprobs_gradient_of_impossible_classes_gpu():
+    from tests.test_lm_ops_cpu import check_gradient_of_impossible_classes
+
+    check_gradient_of_impossible_classes(DEV)
+
+
 def test_logprobs_ties_and_zeros():
     logits = torch.zeros(3, 6000, device=DEV)
     logits[0, 1::2] = -0.0
