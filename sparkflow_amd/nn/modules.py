@@ -184,8 +184,9 @@ class AdapterLinear(nn.Module):
 
     Only the adapters train, so only they are packed, pushed and pulled: at
     rank r a layer sends r (in + out) numbers an adapter and not in * out.
-    ``forward(x, ids)`` takes one adapter a row (negative: none) or the
-    F.adapter_groups of them; without ids every row goes through adapter 0.
+    ``forward(x, ids)`` takes x [..., in_features] and one adapter a row
+    (negative: none), in the leading shape of x, or the F.adapter_groups of
+    them; without ids every row goes through adapter 0.
     B starts at zero, so a new layer answers as its Linear does.
     """
 
@@ -222,7 +223,10 @@ class AdapterLinear(nn.Module):
         if ids is None:
             ids = torch.zeros(x.shape[:-1], dtype=torch.int64,
                               device=x.device)
-        base = F.linear_act(x, self.weight, self.bias, "none")
+        # the dense kernels take contiguous rows of two axes
+        rows = x.reshape(-1, x.shape[-1]).contiguous()
+        base = F.linear_act(rows, self.weight, self.bias, "none")
+        base = base.reshape(x.shape[:-1] + base.shape[1:])
         return F.adapter_add(base, x, self.a, self.b, ids, self.scale,
                              self.activation)
 

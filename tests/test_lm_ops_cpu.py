@@ -387,6 +387,24 @@ def test_adapter_linear_module():
     assert layer.a.grad is not None and x.grad is not None
 
 
+def test_adapter_linear_rows_of_any_shape():
+    from sparkflow_amd import nn as snn
+
+    layer = snn.AdapterLinear(6, 4, 2, adapters=3, activation="relu")
+    with torch.no_grad():
+        layer.b.normal_()
+    x, ids = torch.randn(2, 5, 6), torch.arange(10).reshape(2, 5) % 4 - 1
+    want = layer(x.reshape(10, 6), ids.reshape(10))
+    for leaf in (x.clone(), x.transpose(1, 2).contiguous().transpose(1, 2)):
+        leaf.requires_grad_()
+        got = layer(leaf, ids)
+        torch.testing.assert_close(got, want.reshape(2, 5, 4))
+        got.sum().backward()
+        assert leaf.grad.shape == x.shape
+    torch.testing.assert_close(layer(x[1, 2]), layer(x[:, 2])[1])
+    assert layer(x[:0]).shape == (0, 5, 4)
+
+
 def test_frozen_linear_gradient_of_x():
     for act in ("none", "relu", "sigmoid"):
         x, w, b = torch.randn(5, 6), torch.randn(6, 4), torch.randn(4)

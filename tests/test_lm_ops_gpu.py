@@ -801,6 +801,35 @@ def test_operators_together_gpu(rows):
     check_operators_together(DEV, rows)
 
 
+@pytest.mark.parametrize("act", ["none", "sigmoid"])
+def test_adapter_linear_rows_of_any_shape(act):
+    from sparkflow_amd import nn as snn
+
+    layer = snn.AdapterLinear(12, 7, 3, 4, 0.5, act).to(DEV)
+    with torch.no_grad():
+        layer.b.normal_()
+    x = _randn(2, 5, 12)
+    ids = torch.arange(10, device=DEV).reshape(2, 5) % 5 - 1
+    flat = x.reshape(10, 12).requires_grad_()
+    want = layer(flat, ids.reshape(10))
+    (dw,) = torch.autograd.grad(want.sum(), flat)
+    # three axes; the same from strided rows
+    wide = torch.full((2, 5, 20), math.nan, device=DEV)
+    wide[..., 3:15] = x
+    for leaf in (x.clone().requires_grad_(),
+                 wide[..., 3:15].detach().requires_grad_()):
+        for chosen in (ids, F.adapter_groups(ids, 4)):
+            got = layer(leaf, chosen)
+            assert torch.equal(got, want.reshape(2, 5, 7))
+            (dx,) = torch.autograd.grad(got.sum(), leaf)
+            assert torch.equal(dx, dw.reshape(2, 5, 12))
+    zeros = torch.zeros_like(ids)
+    assert torch.equal(layer(x), layer(x, zeros))
+    assert torch.equal(layer(x[1, 2]), layer(x, zeros)[1, 2])
+    with pytest.raises(RuntimeError, match="shape mismatch"):
+        layer(x.reshape(5, 24), ids.reshape(10)[:5])
+
+
 def test_no_second_derivative():
     """An error, not a silent zero."""
     x = _randn(4, 9).requires_grad_()
