@@ -1108,12 +1108,14 @@ torch::Tensor adapter_plan(torch::Tensor ids, int64_t E) {
   return plan;
 }
 
+// (No rows may have any strides: contiguous() leaves those of an expanded
+// gradient as they are.)
 static void check_rows(const torch::Tensor& t, const char* name, long M,
                        long n, const torch::Tensor& like) {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.dim() == 2 &&
                   t.size(0) == M && t.size(1) == n &&
                   t.scalar_type() == like.scalar_type() &&
-                  (n == 1 || t.stride(1) == 1),
+                  (M == 0 || n == 1 || t.stride(1) == 1),
               name, " must be rows beside the weights, of their type");
 }
 

@@ -692,7 +692,8 @@ __global__ void __launch_bounds__(NT)
 static Tokens check_logits(const torch::Tensor& logits,
                            const torch::Tensor& tokens, int64_t ignore) {
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.size(1) >= 1 &&
-                  (logits.size(1) == 1 || logits.stride(1) == 1) &&
+                  (logits.size(0) == 0 || logits.size(1) == 1 ||
+                   logits.stride(1) == 1) &&
                   logits.size(1) < (1l << 31),
               "logits must be [rows, classes] on GPU with classes side by "
               "side");

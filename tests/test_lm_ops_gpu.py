@@ -695,6 +695,31 @@ def test_adapter_layouts(dtype):
     torch.testing.assert_close(da, de.sum(0, keepdim=True))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_no_rows_of_any_strides(dtype):
+    """Empty batches keep the strides of what they were cut or expanded
+    from, also behind contiguous()."""
+    base, x, a, b, ids, scale = _adapter_inputs(4, 9, 5, 3, 2, dtype=dtype)
+    for cut in (lambda t: t[:0], lambda t: t.t().contiguous().t()[:0],
+                lambda t: t[:1, :1].expand(4, t.shape[1])[:0]):
+        leaves = [cut(t).detach().requires_grad_() for t in (base, x)]
+        leaves += [t.detach().requires_grad_() for t in (a, b)]
+        for act in ("none", "relu"):
+            y = F.adapter_add(*leaves, ids[:0], scale=scale, act=act)
+            assert y.shape == (0, 5)
+            grads = torch.autograd.grad(y.sum(), leaves)  # expanded
+            assert grads[0].shape == (0, 5) and grads[1].shape == (0, 9)
+            assert (grads[2] == 0).all() and (grads[3] == 0).all()
+        r = F.token_logprobs(leaves[1], ids[:0], top_k=2)
+        assert r.logp.shape == (0,) and r.top_ids.shape == (0, 2)
+        (dx,) = torch.autograd.grad(r.logp.sum(), leaves[1])
+        assert dx.shape == (0, 9)
+        state = F.dropout_state(1, device=DEV)
+        y = F.dropout(leaves[1], 0.5, state)
+        (dx,) = torch.autograd.grad(y.sum(), leaves[1])
+        assert y.shape == dx.shape == (0, 9)
+
+
 def test_adapter_partial_gradients_and_groups():
     base, x, a, b, ids, scale = _adapter_inputs(90, 40, 30, 4, 3)
     g = _randn(90, 30, seed=6)
