@@ -355,6 +355,9 @@ static void launch_gemm(const torch::Tensor& A, const torch::Tensor& B,
                         const torch::Tensor& bias, torch::Tensor& C, int M,
                         int N, int K, int lda, int ldb, int act,
                         const float* preY = nullptr, int pre_act = 0) {
+  // an empty batch: a launch without blocks would leave an error behind,
+  // which the next operator reports
+  if (M == 0 || N == 0) return;
   auto stream = at::cuda::getCurrentCUDAStream();
   const bool has_bias = bias.numel() > 0;
   const int splitk = pick_splitk(M, N, K);

@@ -855,6 +855,32 @@ def test_adapter_linear_rows_of_any_shape(act):
         layer(x.reshape(5, 24), ids.reshape(10)[:5])
 
 
+@pytest.mark.parametrize("act", ["none", "relu"])
+def test_layers_on_no_rows(act):
+    """An empty batch is an empty answer, and no launch without blocks whose
+    error the next operator would report."""
+    from sparkflow_amd import nn as snn
+
+    for layer in (snn.AdapterLinear(12, 7, 3, activation=act),
+                  snn.AdapterLinear(300, 7, 3, activation=act, bias=False)):
+        layer.to(DEV)
+        x = torch.empty(0, layer.in_features, device=DEV, requires_grad=True)
+        y = layer(x)
+        assert y.shape == (0, 7)
+        y.sum().backward()
+        assert x.grad.shape == x.shape
+        assert (layer.a.grad == 0).all() and (layer.b.grad == 0).all()
+        assert layer(x.new_empty(3, 0, layer.in_features)).shape == (3, 0, 7)
+    w = _randn(6, 4, seed=1)
+    x = torch.empty(0, 6, device=DEV, requires_grad=True)
+    y = F.linear_act(x, w, None, act)
+    assert y.shape == (0, 4)
+    (dx,) = torch.autograd.grad(y.sum(), x)
+    assert dx.shape == (0, 6)
+    assert F.dropout(torch.ones(4, device=DEV), 0.0,
+                     F.dropout_state(1, device=DEV)).sum() == 4
+
+
 def test_no_second_derivative():
     """An error, not a silent zero."""
     x = _randn(4, 9).requires_grad_()
