@@ -119,29 +119,33 @@ class LinearAct(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        import os
+
         x, w, y = ctx.saved_tensors
         act = ctx.act
         need_dx = ctx.needs_input_grad[0]
         dy = dy.contiguous()
+        fused = os.environ.get("SPARKFLOW_FUSED_ACTBWD", "1") != "0"
         if not (ctx.needs_input_grad[1] or ctx.needs_input_grad[2]):
             # a frozen layer (adapters train beside it): no weight grads
             if not need_dx:
                 return None, None, None, None
             if ops.use_hip(x):
-                dx = ops.hip.gemm_dgrad_act(dy, y, w, act) \
-                    if act != ACT_NONE else ops.hip.gemm_dgrad(dy, w)
+                if act != ACT_NONE and fused:
+                    dx = ops.hip.gemm_dgrad_act(dy, y, w, act)
+                else:
+                    dpre = ops.hip.act_bwd(y, dy, act) \
+                        if act != ACT_NONE else dy
+                    dx = ops.hip.gemm_dgrad(dpre, w)
             else:
                 dx = _act_bwd_from_out(y, dy, act) @ w.t()
             return dx, None, None, None
         if ops.use_hip(x):
-            import os
-
             recs = ctx.defer_sink
             if recs is not None and ctx.has_bias:
                 # deferred-reduce mode: hand the raw split-K workspace to
                 # the fused reduce+apply; weight/bias grads stay None
-                if act != ACT_NONE and \
-                        os.environ.get("SPARKFLOW_FUSED_ACTBWD", "1") != "0":
+                if act != ACT_NONE and fused:
                     dx = ops.hip.gemm_dgrad_act(dy, y, w, act) \
                         if need_dx else None
                     ws = ops.hip.gemm_wgrad_bias_act_ws(x, dy, y, act)
@@ -152,8 +156,7 @@ class LinearAct(torch.autograd.Function):
                     ws = ops.hip.gemm_wgrad_bias_ws(x, dpre)
                 recs.append((w.data_ptr(), ws))
                 return dx, None, None, None
-            if act != ACT_NONE and ctx.has_bias and \
-                    os.environ.get("SPARKFLOW_FUSED_ACTBWD", "1") != "0":
+            if act != ACT_NONE and ctx.has_bias and fused:
                 # activation backward fused into BOTH backward GEMMs'
                 # operand loads — no standalone act_bwd pass or dpre buf
                 dx = ops.hip.gemm_dgrad_act(dy, y, w, act) \

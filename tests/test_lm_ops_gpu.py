@@ -881,6 +881,30 @@ def test_layers_on_no_rows(act):
                      F.dropout_state(1, device=DEV)).sum() == 4
 
 
+@pytest.mark.parametrize("act", ["none", "relu", "sigmoid"])
+def test_frozen_linear_gradient_of_x_gpu(act, monkeypatch):
+    """The same with and without frozen weights, and with the activation's
+    gradient as a kernel of its own (SPARKFLOW_FUSED_ACTBWD=0)."""
+    x, w, b = _randn(33, 20), _randn(20, 17, seed=1), _randn(17, seed=2)
+    g = _randn(33, 17, seed=3)
+
+    def dx(weight, bias):
+        leaf = x.clone().requires_grad_()
+        return torch.autograd.grad(F.linear_act(leaf, weight, bias, act),
+                                   leaf, g)[0]
+
+    want = dx(w.clone().requires_grad_(), b)
+    assert torch.equal(dx(w, b), want) and torch.equal(dx(w, None),
+                                                       dx(w, 0 * b))
+
+    def fused(*args):
+        raise AssertionError("the fused kernel was asked for")
+
+    monkeypatch.setenv("SPARKFLOW_FUSED_ACTBWD", "0")
+    monkeypatch.setattr(ops.hip, "gemm_dgrad_act", fused, raising=False)
+    torch.testing.assert_close(dx(w, b), want)
+
+
 def test_no_second_derivative():
     """An error, not a silent zero."""
     x = _randn(4, 9).requires_grad_()
