@@ -598,6 +598,44 @@ def test_adapter_values(dtype, shape):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [
+    (1, 2048, 64, 16, 1), (7, 20000, 40, 128, 3), (32, 4096, 300, 16, 64),
+    (33, 2500, 129, 12, 5), (64, 4097, 100, 33, 4), (50, 3333, 71, 64, 2)])
+def test_adapter_split_along_inputs(dtype, shape):
+    """Up to 64 rows without gradients: several blocks along the inputs."""
+    base, x, a, b, ids, scale = _adapter_inputs(*shape, dtype=dtype)
+    ids[0] = 0
+    value, tol = oracle.adapter(base, x, a, b, ids, scale)[0]
+    bad = ids.clone()
+    bad[-1] = shape[-1]  # names no adapter
+    with torch.no_grad():
+        y = F.adapter_add(base, x, a, b, ids, scale=scale)
+        _within(y, value, tol)
+        relu = F.adapter_add(base, x, a, b, ids, scale=scale, act="relu")
+        assert torch.equal(relu, torch.relu(y))
+        y2 = F.adapter_add(base, x, a, b, bad, scale=scale)
+        assert torch.isnan(y2[-1]).all() and torch.equal(y2[:-1], y[:-1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [
+    (4096, 136, 72, 32, 3), (4100, 200, 130, 20, 7), (5000, 600, 40, 64, 2),
+    (4097, 33, 65, 17, 40)])
+def test_adapter_two_tiles_a_block(dtype, shape):
+    """From 4096 rows on at ranks of 17 to 64."""
+    _check_adapter(*_adapter_inputs(*shape, dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(8200, 800, 136, 20, 3),
+                                   (8192, 130, 1000, 5, 1),
+                                   (20000, 900, 24, 16, 9)])
+def test_adapter_long_stretches(dtype, shape):
+    """The weights' gradients from more than four tiles a block."""
+    _check_adapter(*_adapter_inputs(*shape, dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m", [60, 2000])
 @pytest.mark.parametrize("ids", ["none", "one", "last", "runs", "absent"])
 def test_adapter_orders(dtype, m, ids):
