@@ -948,8 +948,11 @@ def adapter_add(base, x, a, b, ids, scale=1.0, act="none"):
     x: [..., inputs], what it was given; both are read in place where their
     last axis lies side by side.  a: [adapters, rank, inputs], b: [adapters,
     outputs, rank], all in one type of fp32, bf16 or fp16; sums are 32 bits
-    wide and every result is rounded once.  rank is at most 128, adapters
-    1024; on a GPU rows are less than 2^26.
+    wide and every result is rounded once.  Behind an activation the other
+    gradients start from base's, which is rounded to the type and takes the
+    slope of the rounded output: a sigmoid's where it is nearly 0 or 1 keeps
+    few of its digits in 16 bits.  rank is at most 128, adapters 1024; on a
+    GPU rows are less than 2^26.
 
     ids: one whole number a row (the leading shape of x), or the
     ``adapter_groups`` of them, which the layers of a model share.  A

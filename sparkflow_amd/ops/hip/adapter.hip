@@ -10,7 +10,8 @@
 // by itself), and every kernel works on tiles of up to 16 rows of one
 // adapter, so an adapter is read once a tile and not once a row.  z and dz
 // stay in fp32, [M, Rp] in the grouped order with R padded to 16, 32, 64 or
-// 128: every output is rounded once.
+// 128: every output is rounded once (what an activation adds to that is at
+// adapter_act_bwd).
 //
 // Four kernels do all the products:
 //   shrink  z = s x A^T, dz = s dy B     long sums, few columns
@@ -1038,7 +1039,12 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// d(act) from the output, in the operand's own type.
+// d(act) from the output, in the operand's own type.  Two roundings that
+// other outputs do not have: the slope is that of the rounded y (the sum
+// before it would be another tensor to keep; a sigmoid's slope y (1 - y) is
+// off by up to half a step of y, which is all of it where y rounds to 1),
+// and dy is rounded to the type before dz, dA and dB are taken from it (it is
+// base's gradient, wanted in that type, and the matrix instructions' operand).
 template <typename T>
 __global__ void __launch_bounds__(256)
     adapter_act_bwd_kernel(const T* __restrict__ y, const T* __restrict__ dy,

@@ -696,6 +696,48 @@ def test_adapter_act(dtype, act):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ["relu", "sigmoid"])
+@pytest.mark.parametrize("m", [50, 200, 1500])
+def test_adapter_act_gradients_in_64_bits(dtype, act, m):
+    """Against the gradients of the sum that no one rounded, with the two
+    roundings behind an activation in the bound: the slope is taken from the
+    rounded output, and its product with g is rounded to the type."""
+    base, x, a, b, ids, _ = _adapter_inputs(m, 90, 77, 6, 4, dtype=dtype,
+                                            seed=60)
+    leaves = [t.requires_grad_() for t in (base, x, a, b)]
+    y = F.adapter_add(*leaves, ids, scale=0.25, act=act)
+    g = _randn(m, 77, dtype=dtype, seed=9)
+    got = torch.autograd.grad(y, leaves, g)
+    (pre, tol), = oracle.adapter(base, x, a, b, ids, 0.25)
+    g, half = g.double().cpu(), oracle.half_step(dtype)
+    if act == "relu":
+        slope = (pre > 0).double()
+        off = (pre.abs() <= tol).double()  # either side of 0
+    else:
+        out = torch.sigmoid(pre)
+        slope = out * (1 - out)
+        off = tol + 8 * oracle.U32 + out * half * 1.01
+        off = off + off * off  # d(y - y^2) <= |dy| + dy^2
+    d = g * slope
+    err = g.abs() * (off + (slope + off) * (4 * oracle.U32 + half * 1.01))
+    if dtype == torch.float16:
+        err = err + 2.0 ** -25
+    _within(got[0], d, err)
+    want = oracle.adapter(base, x, a, b, ids, 0.25, d)
+    # what err becomes on its way; 1.01 for its products with the roundings
+    # that the oracle's own bounds hold
+    chosen = (ids.cpu().unsqueeze(1) == torch.arange(4)).double()
+    xa, aa, ba = (t.detach().cpu().double().abs() for t in (x, a, b))
+    dz = 0.25 * torch.einsum("me,mn,enr->mr", chosen, err, ba)
+    z = 0.25 * torch.einsum("me,mk,erk->mr", chosen, xa, aa)
+    more = (torch.einsum("me,mr,erk->mk", chosen, dz, aa),
+            torch.einsum("me,mr,mk->erk", chosen, dz, xa),
+            torch.einsum("me,mn,mr->enr", chosen, err, z))
+    for value, (exact, bound), extra in zip(got[1:], want[1:], more):
+        _within(value, exact, bound + extra * 1.01)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_adapter_layouts(dtype):
     base, x, a, b, ids, scale = _adapter_inputs(48, 65, 33, 5, 3,
                                                 dtype=dtype)
