@@ -151,6 +151,11 @@ class Dropout(nn.Module):
     builder, so every worker of a job draws the same sequence from it;
     ``reseed`` starts another.  Without one, torch's generator and a stored
     mask are used.
+
+    A forward that is run again to save memory (torch.utils.checkpoint, which
+    winds back torch's generator and not this one) would draw another mask
+    for its backward: take the state outside, ``F.dropout_next(rng_state)``,
+    and call F.dropout with it inside.
     """
 
     def __init__(self, p: float = 0.5, seed: int = None):

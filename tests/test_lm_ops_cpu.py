@@ -341,6 +341,30 @@ def test_dropout_module_with_a_seed():
         old.reseed(1)
 
 
+def check_dropout_run_again(device):
+    """A recomputed forward draws the mask of the state that it is given."""
+    from torch.utils.checkpoint import checkpoint
+
+    from sparkflow_amd import nn as snn
+
+    drop = snn.Dropout(0.5, seed=4).to(device)
+    x = torch.ones(64, device=device, requires_grad=True)
+    masks = []
+    for _ in range(2):
+        state = F.dropout_next(drop.rng_state)
+        y = checkpoint(lambda t: F.dropout(t, drop.p, state) ** 2, x,
+                       use_reentrant=False)
+        (dx,) = torch.autograd.grad(y.sum(), x)
+        assert torch.equal(dx, 2 * y)  # 2 x / (1 - p)^2 = 8 where y is 4
+        masks.append(y != 0)
+    assert not torch.equal(*masks)
+    assert drop.rng_state.tolist() == [4, 2]
+
+
+def test_dropout_run_again():
+    check_dropout_run_again("cpu")
+
+
 def _seeded_dropout_mlp():
     from sparkflow_amd.models import dropout_mlp
 

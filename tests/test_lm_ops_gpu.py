@@ -167,6 +167,12 @@ def test_dropout_state_steps_and_captures():
     assert state.tolist()[1] == 5
 
 
+def test_dropout_run_again_gpu():
+    from tests.test_lm_ops_cpu import check_dropout_run_again
+
+    check_dropout_run_again(DEV)
+
+
 def test_dropout_on_another_stream():
     state = F.dropout_state(3, device=DEV)
     x = _randn(100000)
