@@ -801,7 +801,8 @@ def token_logprobs(logits, tokens, top_k: int = 0,
     equal logits the lower class is the better one.
 
     * A row whose token is ``ignore_index`` is not read: zeros, top ids
-      of -1, and a gradient of zero.
+      of -1, and a gradient of zero.  A mean over rows has to leave the
+      ignored ones out.
     * A token outside 0 .. classes - 1 cannot be refused without waiting
       for the device: its log-probability is NaN, and so is its row of the
       gradient if one flows from there.

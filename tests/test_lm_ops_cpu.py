@@ -142,6 +142,20 @@ def test_logprobs_agrees_with_softmax_xent():
     torch.testing.assert_close(x.grad, y.grad)
 
 
+def test_logprobs_loss_leaves_ignored_rows_out():
+    """The loss of the README: the mean over the rows that are read."""
+    logits, labels = torch.randn(12, 10), torch.randint(0, 10, (12,))
+    labels[::3] = -100
+    x, y = (logits.clone().requires_grad_() for _ in range(2))
+    logp = F.token_logprobs(x, labels, ignore_index=-100).logp
+    loss = -logp.sum() / (labels != -100).sum()
+    ref = torch.nn.functional.cross_entropy(y, labels, ignore_index=-100)
+    torch.testing.assert_close(loss, ref)
+    loss.backward()
+    ref.backward()
+    torch.testing.assert_close(x.grad, y.grad)
+
+
 def check_gradient_of_impossible_classes(device):
     """What flows to a named class reaches its logit, possible or not; the
     others' probabilities are 0 and add nothing."""
