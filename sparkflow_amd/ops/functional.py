@@ -670,8 +670,8 @@ def dropout(x, p: float, state, training: bool = True):
     An element is kept with probability 1 - p and scaled by 1 / (1 - p); a
     dropped one is 0 whatever it held.  The same state gives the same mask
     for the same number of elements, on any device, in any type.  x: fp32,
-    bf16 or fp16, any shape; other layouts than contiguous are copied.
-    Without ``training``, or with p = 0, x comes back as it is.
+    bf16 or fp16, any shape, on a GPU less than 64 GiB; other layouts than
+    contiguous are copied.  Without ``training``, or with p = 0, x comes back as it is.
     """
     _check_float("x", x)
     if not 0.0 <= p <= 1.0:
@@ -798,7 +798,8 @@ def token_logprobs(logits, tokens, top_k: int = 0,
     padded vocabulary).  tokens: the leading shape of logits, or that with
     a last extent of 1 (the engine's labels); whole numbers in an integer
     type or fp32.  ``top_k`` is at most 32 and the number of classes; of
-    equal logits the lower class is the better one.
+    equal logits the lower class is the better one.  On a GPU rows are less
+    than 2^24, with up to 1024 classes 2^26.
 
     * A row whose token is ``ignore_index`` is not read: zeros, top ids
       of -1, and a gradient of zero.  A mean over rows has to leave the
