@@ -671,7 +671,8 @@ def dropout(x, p: float, state, training: bool = True):
     dropped one is 0 whatever it held.  The same state gives the same mask
     for the same number of elements, on any device, in any type.  x: fp32,
     bf16 or fp16, any shape, on a GPU less than 64 GiB; other layouts than
-    contiguous are copied.  Without ``training``, or with p = 0, x comes back as it is.
+    contiguous are copied.  Without ``training``, or with p = 0, x comes
+    back as it is.
     """
     _check_float("x", x)
     if not 0.0 <= p <= 1.0:

@@ -115,7 +115,9 @@ __device__ __forceinline__ unsigned long same_group(int g, int bits) {
 // bound by latency on its one CU: a wave loads 8 x 64 ids ahead of using
 // them, and ranks 64 rows at once, by a ballot for each bit of the group (a
 // loop over the groups present: 38 us for 9.9 at 8192 rows of 8 adapters;
-// 300 rows: 4.2 us).  Layers that share their rows share it: adapter_groups.
+// 300 rows: 4.2 us).  A wave holds the ranks of 8 x 64 rows; from 8193 rows
+// on every id is loaded and ranked a second time (8256 rows 14.3 us, 65536
+// 72, 2^20 1.1 ms).  Layers that share their rows share it: adapter_groups.
 __global__ void __launch_bounds__(PLAN_WAVES* WAVE)
     adapter_plan_kernel(Plan p, int tiles, int blocks, int waves) {
   extern __shared__ int hist[];  // [waves][E + 2] and three of [E + 3]
@@ -269,7 +271,8 @@ __device__ __forceinline__ f32x4 mma(Vec<f16_t>::V a, Vec<f16_t>::V b,
 // bf16 has the exponents of fp32, so three of them hold an fp32 number's 24
 // bits exactly: products of z with bf16 weights or rows go through the bf16
 // instruction three times at an eighth of the fp32 instruction's time each.
-// (fp16 has not the exponents: its products are taken in fp32.)
+// (fp16 has not the exponents: three of them would hold z only after a
+// scaling of each row, and its products are taken in fp32.)
 struct Split {
   Vec<bf16_t>::V high, mid, low;
 };
@@ -1202,9 +1205,17 @@ torch::Tensor adapter_shrink(torch::Tensor x, torch::Tensor w,
     for_rank(R, [&](auto rb) {
       constexpr int RB = decltype(rb)::value;
       // Loads of 16 bytes that a lane has in flight: U (1 + RB).  Two tiles
-      // a block halve the reads of W: at 8192 rows of 4096 bf16 and a rank
-      // of 32 that is 18.8 us for 25.5, at 16 25.8 for 17.9 (half as many
-      // blocks are left, and what a CU has under way is what bounds it).
+      // a block halve the reads of W, and the blocks: at 8192 rows of 4096
+      // bf16 and a rank of 32 that is 18.8 us for 25.5, at 16 25.8 for 17.9
+      // (what a CU has under way is what bounds it).  At ranks of 17 to 64
+      // it gains from 4096 rows on, where the tiles are more than the 256
+      // CUs.  z of 4096 inputs, 8 adapters, two tiles for one, us: 3000 rows
+      // bf16 18.9 for 15.0 (rank 32) and 26.7 for 23.1 (64), fp32 36 for 26
+      // and 59 for 47; 4096 rows 18.7 for 24.4, 29 for 42, 38 for 50 and 62
+      // for 91; 16384 rows 58 for 65, 77 for 101, 112 for 116 and 183 for
+      // 207.  It loses where 4096 rows are 256 tiles and no more (one
+      // adapter, rank 32: bf16 18.7 for 16.0, fp32 35 for 26), and in fp32
+      // at 8192 rows and a rank of 32 (79 for 74).
       constexpr int U = RB == 1 ? 8 : RB == 2 ? 4 : 2;
       constexpr int MANY = RB <= 4 ? 16 : 8;  // waves whose sums fit the LDS
       auto go = [&](auto kernel, int waves, long blocks) {
@@ -1320,10 +1331,17 @@ std::vector<torch::Tensor> adapter_outer(c10::optional<torch::Tensor> x,
   const long M = p.M;
   const at::cuda::CUDAGuard guard(like.device());
   auto stream = at::cuda::getCurrentCUDAStream();
-  // Up to 1024 rows one block adds all of an adapter's; above, stretches
-  // that give about 512 blocks, so that one busy adapter is not one block
-  // (8192 rows of 4096 fp16: 44 us, with 256 blocks 54); in bf16, whose
-  // products take less time than its rows' loads, 256 (22 us, with 512 24).
+  // Up to 1024 rows one block adds all of an adapter's, a column chunk each;
+  // above, stretches that give about 512 blocks, so that one busy adapter is
+  // not one block (8192 rows of 4096 fp16: 44 us, with 256 blocks 54); in
+  // bf16, whose products take less time than its rows' loads, 256 (22 us,
+  // with 512 24).  Both weights' gradients, one block for stretches and
+  // their reduce, us.  8 adapters, 784 -> 256 at a rank of 8, fp32: 1024
+  // rows 8.3 for 9.3, 2048 11.8 for 13.0, 4096 19 for 15; 4096 -> 2048 at
+  // 32, bf16: 1024 rows 11 for 21, 4096 17 for 25.  What decides is an
+  // adapter's rows, and a limit by all rows is late for one adapter (784 ->
+  // 256 fp32: 256 rows 7.5 for 8.4, 512 11.0 for 9.4, 1024 29 for 12) and
+  // early for many (64 of them, 4096 rows: 9.8 for 16).
   const bool small = M <= SMALL_ROWS, direct = M <= 1024;
   const long wanted = like.scalar_type() == torch::kBFloat16 ? 256 : 512;
   const long cols = 16 * (like.element_size() == 4 ? 4 : 8);

@@ -287,9 +287,9 @@ __device__ __forceinline__ void write_top(const RowOut& o, long row, int k,
 // behind the last whole vector.
 //
 // In bf16 about nine instructions and an exponential an element keep the
-// vector units 73% busy: 3277 rows of 32000 (210 MB) take 55 us, 3.8 TB/s,
+// vector units 73% busy: 3277 rows of 32000 (210 MB) take 56 us, 3.7 TB/s,
 // where a plain read takes 33; fp32, 461 rows of 50001 with 5 alternatives
-// (92 MB): 20 us, 4.6 TB/s.  Longer rounds, blocks of 128, 512 or 1024
+// (92 MB): 21 us, 4.4 TB/s.  Longer rounds, blocks of 128, 512 or 1024
 // threads and loads before the row's token is known change that by less
 // than 3%.
 template <typename T, int NT, int UNROLL, bool TOP>
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(NT)
 #define SPLITS_MAX 64
 
 // Joins the splits of a row, one wave a row: latency alone (16 rows of 32
-// splits with 20 alternatives 6.4 us, 9.1 before its loads were made to wait
+// splits with 20 alternatives 6.9 us, 9.1 before its loads were made to wait
 // together).  Lane l holds split l and its
 // sorted list.  If q is how many a list has to give on average, c lists
 // whose q-th elements are the largest hold k elements that reach the
@@ -595,7 +595,7 @@ struct RowGrad {
 // of them costs one comparison per listed place, and a span that holds none
 // costs nothing.  Bound by memory: bf16 4096 x 32000, a fifth of the rows
 // ignored (read 210 MB, written 262) 71 us, 6.6 TB/s; fp32 512 x 50001
-// 31 us, 6.2 TB/s.
+// 32 us, 6.1 TB/s.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT)
     logprobs_bwd_kernel(const T* __restrict__ logits, long stride,
