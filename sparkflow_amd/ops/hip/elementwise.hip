@@ -242,6 +242,7 @@ torch::Tensor act_bwd(torch::Tensor y, torch::Tensor dy, int64_t act) {
   check_f32e(dy, "dy");
   auto dpre = torch::empty_like(dy);
   const long n = dy.numel();
+  if (n == 0) return dpre;  // no launch without blocks
   const int blocks = (int)std::min<long>(4096, (n + 255) / 256);
   hipLaunchKernelGGL(act_bwd_kernel, dim3(blocks), dim3(256), 0,
                      at::cuda::getCurrentCUDAStream(), y.data_ptr<float>(),

@@ -991,6 +991,29 @@ def test_frozen_linear_gradient_of_x_gpu(act, monkeypatch):
     torch.testing.assert_close(dx(w, b), want)
 
 
+@pytest.mark.parametrize("act", ["none", "relu", "sigmoid"])
+@pytest.mark.parametrize("fused", ["0", "1"])
+def test_trained_layers_on_no_rows(act, fused, monkeypatch):
+    """Weights' gradients of an empty batch are zero by every route."""
+    monkeypatch.setenv("SPARKFLOW_FUSED_ACTBWD", fused)
+    for bias in (True, False):
+        x = torch.empty(0, 70, device=DEV, requires_grad=True)
+        w = _randn(70, 9, seed=1).requires_grad_()
+        b = _randn(9, seed=2).requires_grad_() if bias else None
+        leaves = [x, w, b] if bias else [x, w]
+        y = F.linear_act(x, w, b, act)
+        grads = torch.autograd.grad(y.sum(), leaves)
+        assert grads[0].shape == (0, 70)
+        assert all((g == 0).all() for g in grads[1:])
+        y = F.linear_act(x, w.detach(), None if b is None else b.detach(),
+                         act)
+        (dx,) = torch.autograd.grad(y.sum(), x)
+        assert dx.shape == (0, 70)
+        # nothing is left behind, nor on the engine's own thread
+        z = torch.ones(4, device=DEV, requires_grad=True)
+        assert torch.autograd.grad((z * z).sum(), z)[0].sum() == 8
+
+
 def test_no_second_derivative():
     """An error, not a silent zero."""
     x = _randn(4, 9).requires_grad_()
