@@ -229,9 +229,10 @@ class AdapterLinear(nn.Module):
             ids = torch.zeros(x.shape[:-1], dtype=torch.int64,
                               device=x.device)
         # the dense kernels take contiguous rows of two axes
-        rows = x.reshape(-1, x.shape[-1]).contiguous()
-        base = F.linear_act(rows, self.weight, self.bias, "none")
-        base = base.reshape(x.shape[:-1] + base.shape[1:])
+        rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+        base = F.linear_act(rows.contiguous(), self.weight, self.bias, "none")
+        if x.dim() != 2:
+            base = base.reshape(x.shape[:-1] + base.shape[1:])
         return F.adapter_add(base, x, self.a, self.b, ids, self.scale,
                              self.activation)
 
