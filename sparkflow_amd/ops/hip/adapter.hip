@@ -449,7 +449,11 @@ __global__ void __launch_bounds__(WAVES * WAVE)
 // compile time: 32 divisions of a sigmoid and the base are registers of a
 // fourth wave a SIMD (out of 8192 rows of 4096 alone, 67 MB, at a rank of 32:
 // 21.1 us for 25.4).  Lanes that trade places, for 128 bytes of a
-// row an instruction, and 1024 or 4096 blocks measured no better.
+// row an instruction, and 1024 or 4096 blocks measured no better.  Few rows
+// at high ranks: a wave alone keeps a whole chunk of W in registers, up to
+// 480, so one wave a SIMD is left (32 rows x 4096 of 64 adapters, ranks of
+// 16, 32, 64 and 128: bf16 5.6, 5.7, 7.9 and 15 us, fp32 5.2, 6.5, 17 and
+// 30).
 template <typename T, int RB, bool RMAJOR, bool SIGMOID, int WAVES>
 __global__ void __launch_bounds__(WAVES * WAVE)
     adapter_expand_kernel(const T* __restrict__ base, long bstride,

@@ -466,7 +466,9 @@ __global__ void __launch_bounds__(NT)
   }
   // More than the list holds: many equal values, or the large ones together
   // in few threads' vectors.  Take them one after another, the largest below
-  // the last.
+  // the last: a pass over the owners' elements each (512 rows of 50001 equal
+  // fp32 logits 214 us with 5 alternatives and 666 with 20, where different
+  // ones take 21 and 26, and whole numbers up to 4 52 and 58).
   unsigned long last = ~0ul;
   for (int j = 0; j < k; ++j) {
     unsigned long top = 0;
