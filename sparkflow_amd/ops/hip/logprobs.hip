@@ -76,7 +76,9 @@ __device__ __forceinline__ Stat wave_join(Stat a) {
 // ref log2 e is rounded before it becomes a whole number, by half a step of
 // fp32: 1/16 at 2^20, but 512 at a mask of -1e10, whose exponential would be
 // infinite or 0.  From 2^20 on, and for an infinity, the sums are therefore
-// about ref itself.
+// about ref itself, at one instruction more an element (4096 rows of 32000
+// bf16, all but 100 of them masked: 52.7 us for 45.9 if the mask is -1e9 and
+// not -1e5; half of them 49.0 for 46.3).
 struct Run {
   float m, ref, limit, shift, s0, s1, t0, t1;
 
@@ -87,6 +89,20 @@ struct Run {
 
   static __device__ __forceinline__ bool far(float ref) {
     return !(fabsf(ref) < 0x1p20f);
+  }
+
+  // Adds 2^d to the sums of j's parity.
+  __device__ __forceinline__ void add(int j, float d) {
+    const float e = __builtin_amdgcn_exp2f(d);
+    // -inf: e is 0 and must meet a finite factor
+    const float f = fmaxf(d, -1000.0f);
+    if (j % 2 == 0) {
+      s0 += e;
+      t0 = fmaf(e, f, t0);
+    } else {
+      s1 += e;
+      t1 = fmaf(e, f, t1);
+    }
   }
 
   // Adds n values.
@@ -118,32 +134,14 @@ struct Run {
       }
     }
     if (far(ref)) {
+      // nothing but -inf so far: it stays -inf, and a NaN a NaN
+      const float about = ref == -INFINITY ? 0.0f : ref;
 #pragma unroll
-      for (int j = 0; j < n; ++j) {
-        // nothing but -inf so far: only a NaN says anything
-        const float d = ref == -INFINITY
-                            ? (x[j] != x[j] ? x[j] : -INFINITY)
-                            : (x[j] - ref) * LOG2E;
-        const float e = __builtin_amdgcn_exp2f(d);
-        s0 += e;
-        t0 = fmaf(e, fmaxf(d, -1000.0f), t0);
-      }
+      for (int j = 0; j < n; ++j) add(j, (x[j] - about) * LOG2E);
       return;
     }
 #pragma unroll
-    for (int j = 0; j < n; ++j) {
-      const float d = fmaf(x[j], LOG2E, -shift);
-      const float e = __builtin_amdgcn_exp2f(d);
-      // -inf: e is 0 and must meet a finite factor
-      const float f = fmaxf(d, -1000.0f);
-      if (j % 2 == 0) {
-        s0 += e;
-        t0 = fmaf(e, f, t0);
-      } else {
-        s1 += e;
-        t1 = fmaf(e, f, t1);
-      }
-    }
+    for (int j = 0; j < n; ++j) add(j, fmaf(x[j], LOG2E, -shift));
   }
 
   // The same about m, in natural steps.  t - s d takes the distance from
